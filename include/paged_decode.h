@@ -334,6 +334,127 @@ int pd_table_from_csr(const int32_t* indptr, const int32_t* indices, int64_t ind
                       int batch, int table_width, int page_size, int max_context, void* stream);
 
 /*
+ * Head norms and position rotation, the step between a model's projections
+ * and its attention. For a head x of head_dim dims at position p:
+ *   y = x / sqrt(mean(x^2) + eps) * w                        (w given)
+ *   (y_a, y_b) <- scale (y_a cos t - y_b sin t, y_a sin t + y_b cos t)
+ * with t = p * frequencies[i] for each pair i of the first rotary_dim dims:
+ * (a, b) = (i, i + rotary_dim / 2) with PD_ROTATE_HALF, (2 i, 2 i + 1) with
+ * PD_ROTATE_INTERLEAVED. Dims from rotary_dim on are not rotated. Everything is
+ * computed in FP32 (the angle in FP64) and rounded once. rotary_dim is a
+ * multiple of 16 up to head_dim, or 0 (norms only; frequencies unused).
+ * Weights are [head_dim], or [heads, head_dim] with *_weight_per_head; NULL: no
+ * norm. weight_dtype is the tokens' dtype or PD_DTYPE_F32. frequencies and the
+ * weights are device memory, weights aligned to 16 bytes; the struct itself is
+ * read during the call. No counterpart in the reference, whose q and cache
+ * rows arrive rotated (docs/DESIGN.md:10-13).
+ */
+enum pd_rotate_style { PD_ROTATE_HALF = 0, PD_ROTATE_INTERLEAVED = 1 };
+
+typedef struct pd_rotation {
+    const double* frequencies;    /* [rotary_dim / 2], radians per position */
+    int rotary_dim;
+    int style;                    /* enum pd_rotate_style */
+    float scale;                  /* factor on cos and sin; 1 for a plain rotation */
+    const void* q_weight;
+    const void* k_weight;
+    int weight_dtype;
+    int q_weight_per_head, k_weight_per_head;
+    float eps;
+} pd_rotation;
+
+/* Rows [batch, tokens, heads, head_dim] of new tokens, strides in elements:
+ * heads are contiguous, tokens and sequences may lie apart (a view of a fused
+ * projection). data is aligned to 16 bytes, strides are multiples of 16 bytes,
+ * not negative. */
+typedef struct pd_token_rows {
+    const void* data;
+    int64_t batch_stride, token_stride;
+} pd_token_rows;
+
+/*
+ * Norms and rotates the heads of q [batch, tokens, query_heads, head_dim] and,
+ * unless k is NULL, k [batch, tokens, kv_heads, head_dim] into the contiguous
+ * q_out and k_out (F32, F16 or BF16, one dtype throughout; an output may be its
+ * own contiguous input). positions is [batch] (token j of sequence b at
+ * positions[b] + j), or [batch, tokens] if positions_per_token is not 0.
+ * batch, tokens, heads <= 65535; head_dim 64 or 128.
+ */
+int pd_rotate_heads(const pd_rotation* rotation, const pd_token_rows* q, const pd_token_rows* k, int dtype,
+                    const int32_t* positions, int positions_per_token, void* q_out, void* k_out, int batch, int tokens,
+                    int query_heads, int kv_heads, int head_dim, void* stream);
+
+/*
+ * pd_append_kv with the keys normed and rotated on the way, from strided rows.
+ * Token j of sequence b is rotated at, and written to, position
+ * positions[b] + j; tokens j >= counts[b] (device int32 [batch], clamped to
+ * [0, tokens]; NULL: all are live) and tokens that map to no valid cache row
+ * (as in pd_append_kv) write nothing. q (or NULL) is normed and rotated at the
+ * same positions into q_out [batch, tokens, query_heads, head_dim], whose rows
+ * j >= counts[b] become zeros. cache_dtype is dtype, or an FP8 format under an
+ * F16 or BF16 dtype: then the cache holds k / k_scale and v / v_scale, rounded
+ * to nearest even, saturated at the largest finite value (NaN stays NaN);
+ * scales are 1 otherwise.
+ */
+int pd_append_rotated(const pd_rotation* rotation, const pd_token_rows* q, const pd_token_rows* k,
+                      const pd_token_rows* v, int dtype, const int32_t* table, const int32_t* positions,
+                      const int32_t* counts, void* q_out, void* k_cache, void* v_cache, int cache_dtype, float k_scale,
+                      float v_scale, int batch, int tokens, int query_heads, int kv_heads, int head_dim, int page_size,
+                      int table_width, int physical_pages, void* stream);
+
+/*
+ * As pd_append_rotated at positions[b] = lengths[b], all or nothing per
+ * sequence as in pd_append_kv_advance (its counts[b] live tokens), and then
+ * lengths[b] grows by counts[b]. q is rotated at lengths[b] + j whether or not
+ * the sequence fits.
+ */
+int pd_append_rotated_advance(const pd_rotation* rotation, const pd_token_rows* q, const pd_token_rows* k,
+                              const pd_token_rows* v, int dtype, const int32_t* table, int32_t* lengths,
+                              const int32_t* counts, void* q_out, void* k_cache, void* v_cache, int cache_dtype,
+                              float k_scale, float v_scale, int batch, int tokens, int query_heads, int kv_heads,
+                              int head_dim, int page_size, int table_width, int physical_pages, int max_context,
+                              void* stream);
+
+/*
+ * Attention of several tokens per sequence over the paged cache: a chunk of a
+ * prompt, drafted tokens, or a decoder's tokens over an encoder's states.
+ *   q, out [batch, tokens, query_heads, head_dim]   F32, F16 or BF16 (out as q)
+ * Sequence b has c_b = counts[b] live tokens (device int32 [batch], clamped to
+ * [0, tokens]; NULL: all). With causal != 0 they are the last ones of its
+ * lengths[b] cache tokens: token j sits at lengths[b] - c_b + j and sees the
+ * tokens up to itself; with causal == 0 every token sees all lengths[b].
+ *   out[b, j, h] = softmax(k_scale K q / sqrt(head_dim)) (v_scale V)
+ * over the tokens it sees, through KV head h / (query_heads / kv_heads). Rows
+ * j >= c_b and rows that see no token are zeros. Formats, page ids and limits
+ * as in pd_decode_ex; tokens <= 65535. Scores, softmax statistics and sums are
+ * FP32; the weights enter the second product in q's type.
+ *
+ * workspace: NULL, or device memory of workspace_bytes (aligned to 16 bytes)
+ * for the states of contexts that are split over workgroups, which few query
+ * rows over long contexts need to fill the device; with less than
+ * pd_decode_tokens_workspace reports the call splits less and is slower. It
+ * needs no initialisation; calls that overlap must not share one.
+ * length_bounds: NULL, or a HOST array [batch] of upper bounds on the lengths,
+ * read during the call, from which the split is chosen. Bounds below the
+ * device lengths are still correct, only slower. No counterpart in the
+ * reference, which decodes one token per sequence (docs/DESIGN.md:5-13).
+ */
+int pd_decode_tokens(const void* q, int q_dtype, const void* k, const void* v, int kv_dtype, float k_scale,
+                     float v_scale, const int32_t* table, const int32_t* lengths, const int32_t* counts, void* out,
+                     void* workspace, size_t workspace_bytes, int batch, int tokens, int query_heads, int kv_heads,
+                     int head_dim, int page_size, int table_width, int physical_pages, int causal,
+                     const int32_t* length_bounds, void* stream);
+
+/*
+ * Bytes of workspace with which pd_decode_tokens calls of up to `tokens`
+ * tokens and these formats and shapes split as they would with any more, on a device of
+ * compute_units CUs (<= 0: the current device's). Returns 0 for arguments that
+ * pd_decode_tokens rejects.
+ */
+size_t pd_decode_tokens_workspace(int q_dtype, int kv_dtype, int batch, int tokens, int query_heads, int kv_heads,
+                                  int head_dim, int page_size, int table_width, int compute_units);
+
+/*
  * Bytes of numerator + stats for a plan: batch * query_heads * 4 * splits *
  * (head_dim + 2) * 4, the reference's DecodePlan.workspace_bytes
  * (src/paged_decode/runtime.py:71-73, docs/DESIGN.md:69-76). Returns 0 for
@@ -435,7 +556,10 @@ const char* pd_status_string(int status);
  * grids, pd_decode_kernel_split; 15: pd_stream_read, indices_count argument
  * of pd_table_from_csr, pd_decode_launch_plan; 16: shared-prefix items,
  * pd_prefix_runs, pd_decode_prefix, pd_decode_partial_prefix, the
- * prefix_runs argument of pd_decode_launch_plan). PD_ABI_VERSION is the
+ * prefix_runs argument of pd_decode_launch_plan). Functions added since
+ * without touching an earlier one keep the number: pd_rotate_heads,
+ * pd_append_rotated, pd_append_rotated_advance, pd_decode_tokens and
+ * pd_decode_tokens_workspace, which a loader finds by name. PD_ABI_VERSION is the
  * value this header describes; a binding compares it with what the loaded
  * library returns. */
 #define PD_ABI_VERSION 16

@@ -36,6 +36,8 @@ PD_ERR_HINT = 7
 PD_ERR_SCRATCH = 8
 PD_ERR_PREFIX = 9
 PD_SCRATCH_BYTES = 32 << 20
+PD_ROTATE_HALF = 0
+PD_ROTATE_INTERLEAVED = 1
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -51,6 +53,21 @@ class LaunchPlan(ctypes.Structure):
                              "merge_chunk_floats", "merge_xcd_grouped", "merge_state_stride", "shared_prefix_items")]
 
 
+class Rotation(ctypes.Structure):
+    """``pd_rotation`` of the header."""
+    _fields_ = [("frequencies", _P), ("rotary_dim", _I), ("style", _I), ("scale", _F), ("q_weight", _P),
+                ("k_weight", _P), ("weight_dtype", _I), ("q_weight_per_head", _I), ("k_weight_per_head", _I),
+                ("eps", _F)]
+
+
+class TokenRows(ctypes.Structure):
+    """``pd_token_rows`` of the header."""
+    _fields_ = [("data", _P), ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64)]
+
+
+_ROTATION = ctypes.POINTER(Rotation)
+_ROWS = ctypes.POINTER(TokenRows)
+
 PROTOTYPES = {
     "pd_decode": (_I, [_P, _P, _P, _I, _P, _P, _P, _P, _P] + [_I] * 10 + [_P]),
     "pd_decode_ex": (_I, [_P, _I, _P, _P, _I, _F, _F, _P, _P, _P, _P, _P] + [_I] * 11 + [_P, _P]),
@@ -64,6 +81,12 @@ PROTOTYPES = {
     "pd_append_kv": (_I, [_P, _P, _I, _P, _P, _P, _P] + [_I] * 7 + [_P]),
     "pd_append_kv_advance": (_I, [_P, _P, _I, _P, _P, _P, _P] + [_I] * 8 + [_P]),
     "pd_table_from_csr": (_I, [_P, _P, ctypes.c_int64, _P, _P, _P, _P] + [_I] * 4 + [_P]),
+    "pd_rotate_heads": (_I, [_ROTATION, _ROWS, _ROWS, _I, _P, _I, _P, _P] + [_I] * 5 + [_P]),
+    "pd_append_rotated": (_I, [_ROTATION, _ROWS, _ROWS, _ROWS, _I, _P, _P, _P, _P, _P, _P, _I, _F, _F] + [_I] * 8 + [_P]),
+    "pd_append_rotated_advance": (_I, [_ROTATION, _ROWS, _ROWS, _ROWS, _I, _P, _P, _P, _P, _P, _P, _I, _F, _F] +
+                                  [_I] * 9 + [_P]),
+    "pd_decode_tokens": (_I, [_P, _I, _P, _P, _I, _F, _F, _P, _P, _P, _P, _P, ctypes.c_size_t] + [_I] * 9 + [_P, _P]),
+    "pd_decode_tokens_workspace": (ctypes.c_size_t, [_I] * 10),
     "pd_workspace_bytes": (ctypes.c_size_t, [_I] * 4),
     "pd_decode_launch_count": (_I, [_I] * 12 + [_P]),
     "pd_decode_kernel_split": (_I, [_I] * 11 + [_P, _I, _P, _P]),
@@ -76,7 +99,8 @@ PROTOTYPES = {
 
 def load(path=LIBRARY):
     """Load the library and attach the prototypes. Raises OSError if it is
-    absent or reports an ABI version other than ``PD_ABI_VERSION``."""
+    absent, reports an ABI version other than ``PD_ABI_VERSION`` or lacks a
+    function that was added since."""
     lib = ctypes.CDLL(str(path))
     lib.pd_abi_version.restype = ctypes.c_int
     lib.pd_abi_version.argtypes = []
@@ -85,7 +109,9 @@ def load(path=LIBRARY):
         raise OSError(f"{path} implements paged_decode ABI {version}, these prototypes follow ABI "
                       f"{PD_ABI_VERSION}: rebuild the library (python -m paged_decode._build)")
     for name, (restype, argtypes) in PROTOTYPES.items():
-        fn = getattr(lib, name)
+        fn = getattr(lib, name, None)
+        if fn is None:
+            raise OSError(f"{path} lacks {name}: rebuild the library (python -m paged_decode._build)")
         fn.restype = restype
         fn.argtypes = argtypes
     return lib

@@ -1,0 +1,39 @@
+// Launches of the attention of several tokens, for one q format and head dimension.
+#ifndef PAGED_DECODE_TOKEN_LAUNCH_H
+#define PAGED_DECODE_TOKEN_LAUNCH_H
+
+#include "token_kernels.h"
+
+namespace pd {
+
+int launch_tokens_f32_d64(const TokenParams&, const TokenPlan&, int kv_dtype, hipStream_t);
+int launch_tokens_f32_d128(const TokenParams&, const TokenPlan&, int kv_dtype, hipStream_t);
+int launch_tokens_f16_d64(const TokenParams&, const TokenPlan&, int kv_dtype, hipStream_t);
+int launch_tokens_f16_d128(const TokenParams&, const TokenPlan&, int kv_dtype, hipStream_t);
+int launch_tokens_bf16_d64(const TokenParams&, const TokenPlan&, int kv_dtype, hipStream_t);
+int launch_tokens_bf16_d128(const TokenParams&, const TokenPlan&, int kv_dtype, hipStream_t);
+
+template <typename QT, int KVF, int D>
+int launch_tokens_format(const TokenParams& p, const TokenPlan& plan, hipStream_t stream) {
+    constexpr int KT = sizeof(QT) == 4 ? 32 : 64;
+    hipLaunchKernelGGL((token_kernel<QT, KVF, D, 1, 4, KT>), dim3(static_cast<uint32_t>(plan.workgroups)), dim3(4 * kWave), 0,
+                       stream, p);
+    if (p.splits > 1) {
+        const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens * p.query_heads;
+        hipLaunchKernelGGL((token_merge_kernel<QT, D>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream, p);
+    }
+    return hipGetLastError() == hipSuccess ? PD_OK : PD_ERR_LAUNCH;
+}
+
+template <typename QT, int D>
+int launch_tokens(const TokenParams& p, const TokenPlan& plan, int kv_dtype, hipStream_t stream) {
+    if constexpr (sizeof(QT) == 2) {
+        if (kv_dtype == PD_DTYPE_FP8_E4M3) return launch_tokens_format<QT, PD_DTYPE_FP8_E4M3, D>(p, plan, stream);
+        if (kv_dtype == PD_DTYPE_FP8_E5M2) return launch_tokens_format<QT, PD_DTYPE_FP8_E5M2, D>(p, plan, stream);
+    }
+    return launch_tokens_format<QT, kTokenNative, D>(p, plan, stream);
+}
+
+}  // namespace pd
+
+#endif  // PAGED_DECODE_TOKEN_LAUNCH_H

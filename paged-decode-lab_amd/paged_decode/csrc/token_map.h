@@ -1,0 +1,139 @@
+// Work map of the attention of several tokens per sequence, shared by the
+// device code in token_kernels.h / tokens.hip and the host: which rows and
+// cache tokens a workgroup takes, what a row sees, and where tiles lie in LDS.
+// Plain integer arithmetic (host and gfx950).
+//
+// The query heads of one KV head and the tokens of one sequence are one list
+// of rows: row = token * group + head of the group. A workgroup takes
+// `tile_rows` of them and one split of the sequence's cache tokens.
+#ifndef PAGED_DECODE_TOKEN_MAP_H
+#define PAGED_DECODE_TOKEN_MAP_H
+
+#include <stddef.h>
+
+#include "partition_map.h"
+
+namespace pd {
+
+struct TokenParams {
+    const void* q;
+    const void* k;
+    const void* v;
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* counts;   // or null: every token is live
+    void* out;
+    float* numerator;        // [rows of all tiles, splits, D], splits > 1 only
+    float* stats;            // [rows of all tiles, splits, 2]
+    int batch, tokens;
+    int query_heads, kv_heads, group;
+    int table_width, page_shift, physical_pages;
+    int causal;
+    int splits;              // of each sequence's cache tokens
+    int split_tokens;        // tokens per split where `splits` of them reach the length
+    int tile_rows, row_tiles;
+    uint32_t kv_row_bytes;   // bytes from one cache token to the next: kv_heads * D * element
+    float scale_log2;        // k_scale / sqrt(D) * log2(e)
+    float v_scale;
+};
+
+// Live query tokens and cache tokens of sequence b.
+PD_HD int token_count(const TokenParams& p, int b) {
+    return p.counts ? imin(imax(p.counts[b], 0), p.tokens) : p.tokens;
+}
+
+PD_HD int token_context(const TokenParams& p, int b) {
+    const int64_t reach = static_cast<int64_t>(p.table_width) << p.page_shift;
+    return static_cast<int>(lmin(imax(p.lengths[b], 0), reach));
+}
+
+// Cache tokens that query token j of `count` sees.
+PD_HD int token_sees(int causal, int context, int count, int j) {
+    return causal ? imax(imin(context, context - count + j + 1), 0) : context;
+}
+
+// Tokens per split of a sequence: split_tokens, or more (a multiple of the
+// unit) where the context outgrew what the host knew.
+constexpr int kTokenSplitUnit = 64;
+
+PD_HD int token_split(int splits, int split_tokens, int context) {
+    const int even = (context + splits - 1) / splits;
+    return imax(split_tokens, (even + kTokenSplitUnit - 1) / kTokenSplitUnit * kTokenSplitUnit);
+}
+
+// Workgroup `block` of the launch (one grid dimension of batch * kv_heads *
+// splits * row_tiles): the tiles that see most come first.
+struct TokenCoords {
+    int b, kv_head, split, tile;
+};
+
+PD_HD TokenCoords token_coords(const TokenParams& p, uint32_t block) {
+    const uint32_t unit = block / p.row_tiles;
+    const uint32_t head = unit / p.splits;
+    TokenCoords c;
+    c.tile = p.row_tiles - 1 - static_cast<int>(block - unit * p.row_tiles);
+    c.split = static_cast<int>(unit - head * p.splits);
+    c.b = static_cast<int>(head / p.kv_heads);
+    c.kv_head = static_cast<int>(head - static_cast<uint32_t>(c.b) * p.kv_heads);
+    return c;
+}
+
+// State of row `row` (of the padded rows of all tiles) of (sequence, KV head) in split s.
+PD_HD int64_t token_state(const TokenParams& p, int b, int kv_head, int row, int s) {
+    const int64_t rows = static_cast<int64_t>(p.row_tiles) * p.tile_rows;
+    return ((static_cast<int64_t>(b) * p.kv_heads + kv_head) * rows + row) * p.splits + s;
+}
+
+// Element offset of row `row` of (sequence, KV head) in q and out.
+PD_HD int64_t token_q_row(const TokenParams& p, int b, int kv_head, int token, int head) {
+    return (static_cast<int64_t>(b) * p.tokens + token) * p.query_heads + static_cast<int64_t>(kv_head) * p.group + head;
+}
+
+// 16-byte chunk position of chunk c of tile row r in LDS: chunks of a row are
+// permuted so that neither the reads of one chunk of many rows (K) nor those
+// of pairs of chunks of four rows (V, transposing) meet in a bank.
+template <int kRowBytes>
+PD_HD int token_chunk(int r, int c) {
+    if (kRowBytes == 128) return r * 8 + (c ^ ((((r >> 1) & 3) << 1) | ((r >> 3) & 1)));      // 16-bit, D 64
+    if (kRowBytes == 256) return r * 16 + (c ^ (((r & 7) << 1) | ((r >> 3) & 1)));            // 16-bit D 128, FP32 D 64
+    return r * 32 + (c ^ (r & 15));                                                          // FP32, D 128
+}
+
+// ---------------------------------------------------------------------------
+// Launch planning (host).
+
+struct TokenPlan {
+    int tile_rows, row_tiles;
+    int splits, split_tokens;
+    int64_t workgroups;
+    int64_t states;  // 0 with one split
+};
+
+constexpr int kTokenMinSplit = 256;    // cache tokens per split, at least
+constexpr int kTokenGroupsPerCu = 2;   // workgroups per CU that a split aims at
+
+inline TokenPlan plan_tokens(int batch, int tokens, int query_heads, int kv_heads, int64_t bound, int64_t max_states,
+                             int compute_units) {
+    TokenPlan t{};
+    const int64_t rows = static_cast<int64_t>(tokens) * (query_heads / kv_heads);
+    t.tile_rows = 64;
+    t.row_tiles = static_cast<int>((rows + t.tile_rows - 1) / t.tile_rows);
+    const int64_t units = static_cast<int64_t>(batch) * kv_heads * t.row_tiles;
+    const int64_t wanted = static_cast<int64_t>(compute_units) * kTokenGroupsPerCu;
+    int64_t splits = units < wanted ? (wanted + units - 1) / units : 1;
+    splits = lmin(splits, lmin((bound + kTokenMinSplit - 1) / kTokenMinSplit, max_states / (units * t.tile_rows)));
+    t.splits = 1;
+    t.split_tokens = kTokenSplitUnit;
+    if (splits > 1) {
+        const int64_t even = (bound + splits - 1) / splits;
+        t.split_tokens = static_cast<int>((even + kTokenSplitUnit - 1) / kTokenSplitUnit * kTokenSplitUnit);
+        t.splits = static_cast<int>((bound + t.split_tokens - 1) / t.split_tokens);
+    }
+    t.workgroups = units * t.splits;
+    t.states = t.splits > 1 ? units * t.tile_rows * t.splits : 0;
+    return t;
+}
+
+}  // namespace pd
+
+#endif  // PAGED_DECODE_TOKEN_MAP_H

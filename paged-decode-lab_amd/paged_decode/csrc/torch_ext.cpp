@@ -379,6 +379,210 @@ void stream_read(torch::Tensor a, torch::Tensor b, int64_t a_bytes, int64_t b_by
                                 static_cast<uint32_t*>(sink.data_ptr()), current_stream(a)));
 }
 
+// A rotation and its norm weights, from the optional tensors of a call.
+pd_rotation rotation_of(const c10::optional<torch::Tensor>& frequencies, int64_t style, double scale,
+                        const c10::optional<torch::Tensor>& q_weight, const c10::optional<torch::Tensor>& k_weight,
+                        double eps, const torch::Tensor& like) {
+    pd_rotation r{};
+    r.style = static_cast<int>(style);
+    r.scale = static_cast<float>(scale);
+    r.eps = static_cast<float>(eps);
+    r.weight_dtype = dtype_code(like);
+    if (frequencies.has_value()) {
+        const auto& f = *frequencies;
+        TORCH_CHECK(f.device() == like.device() && f.is_contiguous() && f.scalar_type() == at::kDouble && f.dim() == 1,
+                    "frequencies must be a contiguous float64 tensor on the inputs' device");
+        r.frequencies = f.data_ptr<double>();
+        r.rotary_dim = static_cast<int>(2 * f.numel());
+    }
+    for (const auto* w : {&q_weight, &k_weight}) {
+        if (!w->has_value()) continue;
+        const auto& t = **w;
+        TORCH_CHECK(t.device() == like.device() && t.is_contiguous() && (t.dim() == 1 || t.dim() == 2) &&
+                        t.size(-1) == like.size(3) && dtype_code(t) >= 0 && dtype_code(t) <= PD_DTYPE_BF16,
+                    "norm weights must be contiguous [D] or [H, D] tensors on the inputs' device");
+        r.weight_dtype = dtype_code(t);
+        (w == &q_weight ? r.q_weight : r.k_weight) = t.data_ptr();
+        (w == &q_weight ? r.q_weight_per_head : r.k_weight_per_head) = t.dim() == 2;
+    }
+    return r;
+}
+
+// Strided rows [B, n, H, D]; a dim of one element has no stride of its own.
+pd_token_rows rows_of(const torch::Tensor& t, const torch::Tensor& like) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.dim() == 4 && t.scalar_type() == like.scalar_type() &&
+                    t.size(0) == like.size(0) && t.size(1) == like.size(1) && t.size(3) == like.size(3) &&
+                    t.stride(3) == 1 && (t.size(2) == 1 || t.stride(2) == t.size(3)),
+                "expected rows [B, tokens, heads, D] of one dtype with contiguous heads on one GPU");
+    return {t.data_ptr(), t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0};
+}
+
+// Whether the memory of two tensors overlaps.
+bool overlaps(const torch::Tensor& a, const torch::Tensor& b) {
+    const auto range = [](const torch::Tensor& t) {
+        int64_t last = 0;
+        for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+        const auto begin = reinterpret_cast<uintptr_t>(t.data_ptr());
+        return std::make_pair(begin, begin + static_cast<uintptr_t>((last + 1) * t.element_size()));
+    };
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    const auto x = range(a), y = range(b);
+    return x.first < y.second && y.first < x.second;
+}
+
+// An output of rows `own`: contiguous, and sharing memory with no input but
+// `own` itself, element for element.
+void check_rows_output(const torch::Tensor& out, const torch::Tensor& own,
+                       std::initializer_list<const torch::Tensor*> others) {
+    TORCH_CHECK(out.device() == own.device() && out.is_contiguous() && out.scalar_type() == own.scalar_type() &&
+                    out.numel() == own.numel(),
+                "outputs must be contiguous, of their input's dtype and size, on its device");
+    TORCH_CHECK((out.data_ptr() == own.data_ptr() && own.is_contiguous()) || !overlaps(out, own),
+                "an output may only be its own contiguous input");
+    for (const auto* t : others) TORCH_CHECK(t == nullptr || !overlaps(out, *t), "an output overlaps another tensor of the call");
+}
+
+const torch::Tensor* pointer(const c10::optional<torch::Tensor>& t) { return t.has_value() ? &*t : nullptr; }
+
+// Head norms and rotation of q and, if given, k.
+void rotate_heads(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions, bool per_token,
+                  c10::optional<torch::Tensor> frequencies, int64_t style, double scale,
+                  c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight, double eps,
+                  torch::Tensor q_out, c10::optional<torch::Tensor> k_out) {
+    const pd_token_rows q_rows = rows_of(q, q);
+    pd_token_rows k_rows{};
+    TORCH_CHECK(k.has_value() == k_out.has_value(), "k and its output come together");
+    check_rows_output(q_out, q, {pointer(k), pointer(k_out)});
+    if (k.has_value()) {
+        k_rows = rows_of(*k, q);
+        check_rows_output(*k_out, *k, {&q, &q_out});
+    }
+    TORCH_CHECK(positions.device() == q.device() && positions.is_contiguous() && positions.scalar_type() == at::kInt &&
+                    positions.numel() == (per_token ? q.size(0) * q.size(1) : q.size(0)),
+                "positions must be int32, one per sequence or token, on the inputs' device");
+    const pd_rotation r = rotation_of(frequencies, style, scale, q_weight, k_weight, eps, q);
+    TORCH_CHECK(!r.q_weight_per_head || q_weight->size(0) == q.size(2), "q_weight must be [D] or [H, D]");
+    TORCH_CHECK(!r.k_weight_per_head || (k.has_value() && k_weight->size(0) == k->size(2)), "k_weight must be [D] or [H, D]");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+    check_status(pd_rotate_heads(&r, &q_rows, k.has_value() ? &k_rows : nullptr, dtype_code(q),
+                                 positions.data_ptr<int32_t>(), per_token, q_out.data_ptr(),
+                                 k.has_value() ? k_out->data_ptr() : nullptr, static_cast<int>(q.size(0)),
+                                 static_cast<int>(q.size(1)), static_cast<int>(q.size(2)),
+                                 k.has_value() ? static_cast<int>(k->size(2)) : 0, static_cast<int>(q.size(3)),
+                                 current_stream(q)));
+}
+
+// Paged append of normed and rotated keys and of values; max_context >= 0:
+// positions are lengths, advanced on the device (all or nothing per sequence).
+void append_rotated(c10::optional<torch::Tensor> q, torch::Tensor k_new, torch::Tensor v_new, torch::Tensor table,
+                    torch::Tensor positions, c10::optional<torch::Tensor> counts,
+                    c10::optional<torch::Tensor> frequencies, int64_t style, double scale,
+                    c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight, double eps,
+                    c10::optional<torch::Tensor> q_out, torch::Tensor k_cache, torch::Tensor v_cache, double k_scale,
+                    double v_scale, int64_t max_context) {
+    const pd_token_rows k_rows = rows_of(k_new, k_new), v_rows = rows_of(v_new, k_new);
+    pd_token_rows q_rows{};
+    const int64_t batch = k_new.size(0);
+    for (const auto& t : {k_cache, v_cache, table, positions}) {
+        TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.device() == k_new.device(),
+                    "all tensors must be contiguous GPU tensors on one device");
+    }
+    TORCH_CHECK(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes() && k_cache.size(2) == k_new.size(2) &&
+                    k_cache.size(3) == k_new.size(3) && v_new.sizes() == k_new.sizes() &&
+                    v_cache.scalar_type() == k_cache.scalar_type() && k_cache.size(0) <= INT32_MAX,
+                "expected k/v cache [P,T,KV,D] matching k_new/v_new [B,tokens,KV,D]");
+    TORCH_CHECK(table.dim() == 2 && table.size(0) == batch && positions.dim() == 1 && positions.size(0) == batch &&
+                    table.scalar_type() == at::kInt && positions.scalar_type() == at::kInt,
+                "table must be int32 [B, W] and positions int32 [B]");
+    if (counts.has_value()) {
+        TORCH_CHECK(counts->device() == k_new.device() && counts->is_contiguous() && counts->scalar_type() == at::kInt &&
+                        counts->dim() == 1 && counts->size(0) == batch,
+                    "counts must be int32 [B]");
+    }
+    TORCH_CHECK(!overlaps(k_cache, v_cache), "the caches overlap");
+    for (const auto* cache : {&k_cache, &v_cache})
+        for (const auto* t : {static_cast<const torch::Tensor*>(&k_new), static_cast<const torch::Tensor*>(&v_new), pointer(q), pointer(q_out)})
+            TORCH_CHECK(t == nullptr || !overlaps(*cache, *t), "the cache overlaps another tensor of the call");
+    TORCH_CHECK(q.has_value() == q_out.has_value(), "q and its output come together");
+    if (q.has_value()) {
+        q_rows = rows_of(*q, k_new);
+        check_rows_output(*q_out, *q, {&k_new, &v_new});
+    }
+    const pd_rotation r = rotation_of(frequencies, style, scale, q_weight, k_weight, eps, k_new);
+    TORCH_CHECK(!r.q_weight_per_head || (q.has_value() && q_weight->size(0) == q->size(2)), "q_weight must be [D] or [H, D]");
+    TORCH_CHECK(!r.k_weight_per_head || k_weight->size(0) == k_new.size(2), "k_weight must be [D] or [H, D]");
+    TORCH_CHECK(max_context <= (1 << 20), "max_context must not exceed 1048576");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k_new.device());
+    const pd_token_rows* q_arg = q.has_value() ? &q_rows : nullptr;
+    void* q_dst = q.has_value() ? q_out->data_ptr() : nullptr;
+    const int32_t* count = counts.has_value() ? counts->data_ptr<int32_t>() : nullptr;
+    const int b = static_cast<int>(batch), n = static_cast<int>(k_new.size(1));
+    const int hq = q.has_value() ? static_cast<int>(q->size(2)) : 0, kv = static_cast<int>(k_new.size(2));
+    const int d = static_cast<int>(k_new.size(3)), page = static_cast<int>(k_cache.size(1));
+    const int width = static_cast<int>(table.size(1)), pages = static_cast<int>(k_cache.size(0));
+    const int dtype = dtype_code(k_new), cache_dtype = dtype_code(k_cache);
+    const float ks = static_cast<float>(k_scale), vs = static_cast<float>(v_scale);
+    if (max_context >= 0) {
+        check_status(pd_append_rotated_advance(&r, q_arg, &k_rows, &v_rows, dtype, table.data_ptr<int32_t>(),
+                                               positions.data_ptr<int32_t>(), count, q_dst, k_cache.data_ptr(),
+                                               v_cache.data_ptr(), cache_dtype, ks, vs, b, n, hq, kv, d, page, width,
+                                               pages, static_cast<int>(max_context), current_stream(k_new)));
+    } else {
+        check_status(pd_append_rotated(&r, q_arg, &k_rows, &v_rows, dtype, table.data_ptr<int32_t>(),
+                                       positions.data_ptr<int32_t>(), count, q_dst, k_cache.data_ptr(),
+                                       v_cache.data_ptr(), cache_dtype, ks, vs, b, n, hq, kv, d, page, width, pages,
+                                       current_stream(k_new)));
+    }
+}
+
+// Attention of several tokens per sequence (pd_decode_tokens).
+void decode_tokens(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lengths,
+                   c10::optional<torch::Tensor> counts, torch::Tensor out, torch::Tensor workspace, bool causal,
+                   double k_scale, double v_scale, c10::optional<torch::Tensor> length_bounds) {
+    for (const auto& t : {q, k, v, table, lengths, out, workspace}) {
+        TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.device() == q.device(),
+                    "all tensors must be contiguous GPU tensors on one device");
+    }
+    TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes() && k.size(3) == q.size(3) &&
+                    k.scalar_type() == v.scalar_type() && k.size(0) <= INT32_MAX,
+                "expected q[B,tokens,H,D], k/v[P,T,KV,D]");
+    TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out must be as q");
+    for (const auto* t : {&q, &k, &v}) TORCH_CHECK(!overlaps(out, *t), "out overlaps an input");
+    const int64_t batch = q.size(0);
+    TORCH_CHECK(table.dim() == 2 && table.size(0) == batch && lengths.dim() == 1 && lengths.size(0) == batch &&
+                    table.scalar_type() == at::kInt && lengths.scalar_type() == at::kInt,
+                "table must be int32 [B, W] and lengths int32 [B]");
+    if (counts.has_value()) {
+        TORCH_CHECK(counts->device() == q.device() && counts->is_contiguous() && counts->scalar_type() == at::kInt &&
+                        counts->dim() == 1 && counts->size(0) == batch,
+                    "counts must be int32 [B]");
+    }
+    const int32_t* bounds = bounds_pointer(length_bounds, batch);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+    const size_t bytes = static_cast<size_t>(workspace.numel() * workspace.element_size());
+    check_status(pd_decode_tokens(q.data_ptr(), dtype_code(q), k.data_ptr(), v.data_ptr(), dtype_code(k),
+                                  static_cast<float>(k_scale), static_cast<float>(v_scale), table.data_ptr<int32_t>(),
+                                  lengths.data_ptr<int32_t>(), counts.has_value() ? counts->data_ptr<int32_t>() : nullptr,
+                                  out.data_ptr(), bytes > 0 ? workspace.data_ptr() : nullptr, bytes,
+                                  static_cast<int>(batch), static_cast<int>(q.size(1)), static_cast<int>(q.size(2)),
+                                  static_cast<int>(k.size(2)), static_cast<int>(q.size(3)), static_cast<int>(k.size(1)),
+                                  static_cast<int>(table.size(1)), static_cast<int>(k.size(0)), causal, bounds,
+                                  current_stream(q)));
+}
+
+// Workspace bytes of decode_tokens calls of up to `tokens` tokens, whatever their formats.
+int64_t decode_tokens_workspace(int64_t batch, int64_t tokens, int64_t query_heads, int64_t kv_heads, int64_t head_dim,
+                                int64_t page_size, int64_t table_width) {
+    size_t bytes = 0;
+    for (int q : {PD_DTYPE_F32, PD_DTYPE_F16, PD_DTYPE_BF16})
+        for (int kv : {q, static_cast<int>(PD_DTYPE_FP8_E4M3)})
+            bytes = std::max(bytes, pd_decode_tokens_workspace(q, kv, static_cast<int>(batch), static_cast<int>(tokens),
+                                                               static_cast<int>(query_heads), static_cast<int>(kv_heads),
+                                                               static_cast<int>(head_dim), static_cast<int>(page_size),
+                                                               static_cast<int>(table_width), 0));
+    return static_cast<int64_t>(bytes);
+}
+
 PYBIND11_MODULE(_C, m) {
     m.doc() = "Split-K paged GQA decode for gfx950 (calls libpaged_decode_hip.so)";
     m.def("decode", &decode, "Paged split-K GQA decode (partition + merge)", py::arg("q"), py::arg("k"), py::arg("v"),
@@ -396,6 +600,10 @@ PYBIND11_MODULE(_C, m) {
     m.def("append_kv", &append_kv, "Paged KV-cache append", py::arg("k_new"), py::arg("v_new"), py::arg("table"),
           py::arg("positions"), py::arg("k_cache"), py::arg("v_cache"), py::arg("advance"),
           py::arg("max_context") = -1);
+    m.def("rotate_heads", &rotate_heads, "Head norms and position rotation");
+    m.def("append_rotated", &append_rotated, "Paged KV-cache append of normed and rotated keys");
+    m.def("decode_tokens", &decode_tokens, "Attention of several tokens per sequence over the paged cache");
+    m.def("decode_tokens_workspace", &decode_tokens_workspace, "Workspace bytes of decode_tokens");
     m.def("table_from_csr", &table_from_csr, "CSR page lists to page table and lengths on the device",
           py::arg("indptr"), py::arg("indices"), py::arg("last_page_len"), py::arg("table"), py::arg("lengths"),
           py::arg("overflow") = py::none(), py::arg("page_size"), py::arg("max_context"));

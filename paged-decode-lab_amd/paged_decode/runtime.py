@@ -67,7 +67,7 @@ class DecodePlan:
     """
 
     def __init__(self, layout: Layout, table, lengths, *, device="cuda", split_tokens=256, merge="serial",
-                 max_context=None):
+                 max_context=None, query_tokens=None):
         if merge not in ("serial", "shared"):
             raise ValueError("merge must be 'serial' or 'shared'")
         if layout.head_dim not in (64, 128):
@@ -96,7 +96,11 @@ class DecodePlan:
         self.splits = max(1, math.ceil(capacity / split_tokens))
         if self.splits > 65535:
             raise ValueError("too many context splits")
+        if query_tokens is not None and (isinstance(query_tokens, bool) or not isinstance(query_tokens, int) or
+                                         not 1 <= query_tokens <= 65535):
+            raise ValueError("query_tokens must be an integer in [1,65535]")
         self.layout, self.split_tokens = layout, split_tokens
+        self.query_tokens = query_tokens
         self.merge = merge
         if merge == "shared":
             fits = self.splits * _STATES_PER_SPLIT <= _SHARED_MERGE_MAX_PARTS
@@ -128,6 +132,15 @@ class DecodePlan:
         self._staged_split = (self.splits, split_tokens)
         self._extension = load_extension()
         self._prefix_runs = self._shared_prefixes(table)
+        if query_tokens is not None:
+            # Output and split states of run_tokens, for up to that many tokens of any dtype.
+            shape = (layout.batch, query_tokens, layout.query_heads, layout.head_dim)
+            self._token_out = torch.empty(shape, dtype=torch.float32, device=self.device)
+            with torch.cuda.device(self.device):
+                size = self._extension.decode_tokens_workspace(layout.batch, query_tokens, layout.query_heads,
+                                                               layout.kv_heads, layout.head_dim, layout.page_size,
+                                                               table.shape[1])
+            self._token_workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
 
     @classmethod
     def from_csr(cls, layout: Layout, indptr, indices, last_page_len, **kwargs):
@@ -224,6 +237,31 @@ class DecodePlan:
         if self._bounds_known:
             self._bounds.add_(k_new.shape[1]).clamp_(max=self.context_capacity)
 
+    def append_rotated(self, k_cache, v_cache, k_new, v_new, rotary, *, q=None, q_weight=None, k_weight=None, eps=1e-6,
+                       k_scale=1.0, v_scale=1.0, counts=None, out=None):
+        """``append`` with the new keys normed and rotated on the way, at the plan's current lengths, which it
+        advances on the device; returns the rotated ``q``.
+
+        Arguments as in ``paged_decode.rotary.append_rotated``, positions being
+        the lengths. A sequence is written, and its length advanced by
+        ``counts[b]`` (all tokens without ``counts``), only if all its live
+        tokens fall on valid pages below ``context_capacity``; q is rotated
+        either way. No host synchronisation: it can be captured with ``run``
+        and ``run_tokens``.
+        """
+        from .rotary import launch_append
+
+        if k_new.device != self.device:
+            raise ValueError("cache and new tokens must be contiguous on the plan device")
+        tokens = k_new.shape[1] if k_new.dim() == 4 else 1
+        if tokens > self.context_capacity:
+            raise ValueError("more new tokens than the plan's reserved context")
+        out = launch_append(self.layout, k_cache, v_cache, self._table, self._lengths, k_new, v_new, rotary, q, q_weight,
+                            k_weight, eps, k_scale, v_scale, counts, out, self.context_capacity)
+        if self._bounds_known:
+            self._bounds.add_(tokens).clamp_(max=self.context_capacity)
+        return out
+
     @property
     def workspace_bytes(self):
         """Bytes of the partition-state workspace (numerator + stats)."""
@@ -236,9 +274,7 @@ class DecodePlan:
         if tuple(q.shape) != expected_q or tuple(k.shape) != expected_k or tuple(v.shape) != expected_k:
             raise ValueError("input shape does not match plan")
         _check_formats(q.dtype, k.dtype, v.dtype)
-        for scale in (k_scale, v_scale):
-            if isinstance(scale, bool) or not isinstance(scale, (int, float)) or not 0 < scale < math.inf:
-                raise ValueError("k_scale and v_scale must be finite and positive")
+        check_scales(k_scale, v_scale)
         for tensor in (q, k, v):
             if tensor.device != self.device or not tensor.is_contiguous():
                 raise ValueError("inputs must be contiguous on the plan device")
@@ -258,6 +294,48 @@ class DecodePlan:
                                self._out, self.split_tokens, self._merge_mode, float(k_scale), float(v_scale),
                                self._unshared_pages, self._ragged_lengths, self._length_bounds(), self._prefix_runs)
         return self._out
+
+    def run_tokens(self, q, k, v, *, causal=True, counts=None, k_scale=1.0, v_scale=1.0, out=None):
+        """Attention of several tokens per sequence over the cache; returns ``[B, n, Hq, D]`` in q's dtype.
+
+        ``q`` is ``[B, n, Hq, D]`` with ``n`` up to the plan's ``query_tokens``.
+        With ``causal`` its tokens are the last ones of each sequence's current
+        length (append them first): token ``j`` of the ``c`` that sequence
+        ``b`` brings sits at ``lengths[b] - c + j`` and sees the tokens up to
+        itself, so one call serves a chunk of a prompt, a whole prompt or
+        drafted tokens. Without, every token sees all ``lengths[b]`` (a
+        decoder's tokens over an encoder's states). ``counts`` (int32 ``[B]`` on
+        the device) is ``c`` where sequences bring different numbers (default:
+        all ``n``); rows behind are zeros, as are rows that see nothing.
+        Formats and scales as in ``run``; the output is rounded to q's dtype.
+        Without ``out`` (contiguous, q's shape and dtype) the result is the
+        plan's own tensor, overwritten by the next ``run_tokens``.
+        """
+        if self.query_tokens is None:
+            raise ValueError("the plan reserves no query tokens: build it with query_tokens")
+        layout = self.layout
+        expected_k = (layout.physical_pages, layout.page_size, layout.kv_heads, layout.head_dim)
+        if q.dim() != 4 or q.shape[0] != layout.batch or tuple(q.shape[2:]) != (layout.query_heads, layout.head_dim) or \
+                not 1 <= q.shape[1] <= self.query_tokens or tuple(k.shape) != expected_k or tuple(v.shape) != expected_k:
+            raise ValueError("input shape does not match plan")
+        _check_formats(q.dtype, k.dtype, v.dtype)
+        check_scales(k_scale, v_scale)
+        for tensor in (q, k, v) if out is None else (q, k, v, out):
+            if tensor.device != self.device or not tensor.is_contiguous():
+                raise ValueError("inputs must be contiguous on the plan device")
+            if tensor.requires_grad:
+                raise ValueError("inference only: detach tensors requiring gradients")
+        if counts is not None:
+            from .rotary import check_counts
+
+            check_counts(counts, layout.batch, self.device)
+        if out is None:
+            out = self._token_out.view(q.dtype).view(-1)[:q.numel()].view(q.shape)
+        elif out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out must have q's shape and dtype")
+        self._extension.decode_tokens(q, k, v, self._table, self._lengths, counts, out, self._token_workspace,
+                                      bool(causal), float(k_scale), float(v_scale), self._length_bounds())
+        return out
 
     def launches(self, q_dtype, kv_dtype=None):
         """Kernel launches ``run`` makes for q (and K/V) of these dtypes: 1 when the
@@ -403,6 +481,12 @@ def _check_formats(q_dtype, k_dtype, v_dtype):
             k_dtype == q_dtype or (k_dtype in _FP8 and q_dtype != torch.float32)):
         raise TypeError("q/k/v must share float16, bfloat16 or float32 dtype "
                         "(k/v may be float8_e4m3fn/float8_e5m2 with a float16 or bfloat16 q)")
+
+
+def check_scales(k_scale, v_scale):
+    for scale in (k_scale, v_scale):
+        if isinstance(scale, bool) or not isinstance(scale, (int, float)) or not 0 < scale < math.inf:
+            raise ValueError("k_scale and v_scale must be finite and positive")
 
 
 def _check_cache(k_cache, v_cache, k_new, v_new, expected_k, device):
