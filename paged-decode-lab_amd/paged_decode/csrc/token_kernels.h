@@ -13,6 +13,8 @@
 #ifndef PAGED_DECODE_TOKEN_KERNELS_H
 #define PAGED_DECODE_TOKEN_KERNELS_H
 
+#include <utility>
+
 #include "device_common.h"
 #include "token_map.h"
 
@@ -136,14 +138,15 @@ __device__ __forceinline__ void store_row_zeros(const TokenParams& p, const Toke
 // The rows of a tile one by one, a wave each, on the vector units: for tiles
 // in which a token that some rows see and others do not has an infinity or NaN in
 // V, since 0 * V would carry it into the rows that do not see it.
-template <typename QT, int KVF, int D, int WAVES, int M>
-__device__ __forceinline__ void token_rows_one_by_one(const TokenParams& p, const TokenWork& w, int wave, int lane) {
+template <typename QT, int KVF, int D>
+__device__ __forceinline__ void token_rows_one_by_one(const TokenParams& p, const TokenWork& w, int rows, int first, int step,
+                                                      int lane) {
     constexpr int PER = D / kWave;
     constexpr int ES = KVF == kTokenNative ? sizeof(QT) : 1;
     const int32_t* pages = p.table + static_cast<int64_t>(w.b) * p.table_width;
     const char* k_head = static_cast<const char*>(p.k) + static_cast<size_t>(w.kv_head) * D * ES;
     const char* v_head = static_cast<const char*>(p.v) + static_cast<size_t>(w.kv_head) * D * ES;
-    for (int i = wave; i < M; i += WAVES) {
+    for (int i = first; i < rows; i += step) {
         const int row = w.row0 + i;
         if (row >= w.rows) {
             if (p.splits == 1) store_row_zeros<QT, D>(p, w, row, lane);
@@ -187,128 +190,169 @@ __device__ __forceinline__ void token_rows_one_by_one(const TokenParams& p, cons
     }
 }
 
-// A workgroup of WAVES waves, R blocks of 16 rows each, over tiles of KT cache
-// tokens that the waves share through LDS.
-template <typename QT, int KVF, int D, int R, int WAVES, int KT>
-__global__ void __launch_bounds__(kWave * WAVES) token_kernel(const TokenParams p) {
-    constexpr bool kF32 = sizeof(QT) == 4;
-    constexpr int ES = KVF == kTokenNative ? static_cast<int>(sizeof(QT)) : 1;  // stored element
-    constexpr int RB = D * static_cast<int>(sizeof(QT));  // bytes of a tile row in LDS
-    constexpr int CPR = RB / 16;
-    constexpr int NI = KT / 16;         // blocks of 16 cache tokens
-    constexpr int KS = RB / 64;         // steps of four chunks of the first product
-    constexpr int ND = D / 16;          // blocks of 16 dims of the second
-    constexpr int M = WAVES * R * 16;
-    constexpr int CE = 16 / static_cast<int>(sizeof(QT));  // elements of a chunk
-    using Math = TokenMath<QT>;
-    __shared__ __attribute__((aligned(16))) char k_tile[KT * RB];
-    __shared__ __attribute__((aligned(16))) char v_tile[KT * RB];
+// ---------------------------------------------------------------------------
+// Page ids of a tile of KT tokens from t on: lane i holds that of tokens
+// t + 16 i .. + 15. Requested a tile ahead of the rows' own requests, which wait for it.
+template <int KT>
+__device__ __forceinline__ int tile_pages(const TokenParams& p, const int32_t* pages, int t, int lane) {
+    return pages[imin((t + 16 * imin(lane, KT / 16 - 1)) >> p.page_shift, p.table_width - 1)];
+}
 
-    const int lane = threadIdx.x % kWave;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int col = lane % 16, quad = lane / 16;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const char* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, 0x00027000);
+}
 
-    TokenWork w;
-    const TokenCoords at = token_coords(p, blockIdx.x);
-    w.b = at.b;
-    w.kv_head = at.kv_head;
-    w.split = at.split;
-    w.row0 = at.tile * M;
-    w.count = token_count(p, w.b);
-    w.context = token_context(p, w.b);
-    w.rows = w.count * p.group;
-    const int last = imin(w.row0 + M, w.rows) - 1;
-    const int span = token_split(p.splits, p.split_tokens, w.context);
-    w.begin = w.split * span;
-    w.end = last < w.row0 ? 0 : imin(w.begin + span, token_sees(p.causal, w.context, w.count, last / p.group));
-    if (w.begin >= w.end) {  // nothing to see; states of such splits are never read
-        if (p.splits == 1)
-            for (int i = wave; i < M; i += WAVES) store_row_zeros<QT, D>(p, w, w.row0 + i, lane);
-        return;
+// Address of an LDS array within the workgroup's LDS.
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p));
+}
+
+// 16 bytes per lane from a buffer into LDS at to + kOffset + 16 lane, past the
+// registers. In assembly since the compiler, where it knows of such a load, waits for it
+// before the next read of any LDS; here wait_for_loads and a barrier come
+// before the tile's first read. Nothing is returned in registers.
+template <int kOffset>
+__device__ __forceinline__ void load_to_lds(const char* base, uint32_t bytes, uint32_t to, uint32_t offset) {
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    const u32x4 buffer = {static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32) & 0xFFFFu, bytes, 0x00027000u};
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
+                 :
+                 : "s"(to), "i"(kOffset), "v"(offset), "s"(buffer)
+                 : "memory", "scc");
+}
+
+// All loads of this wave but the last kNewer have arrived, those into LDS too.
+template <int kNewer = 0>
+__device__ __forceinline__ void wait_for_loads() {
+    static_assert(kNewer < 64, "the counter's range");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kNewer) : "memory");
+}
+
+// This wave's reads of LDS are done: what they read may be overwritten.
+__device__ __forceinline__ void wait_for_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// The cache rows of 16 tokens from t on (one page): where they start, and the
+// bytes of those before `end` (0 on an invalid page): what lies behind reads as zeros.
+struct RowBlock {
+    int64_t offset;
+    uint32_t bytes;
+};
+
+__device__ __forceinline__ RowBlock row_block(const TokenParams& p, int page, int t, int end) {
+    const bool valid = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.physical_pages) && t < end;
+    const int64_t row = (static_cast<int64_t>(valid ? page : 0) << p.page_shift) + (t & ((1 << p.page_shift) - 1) & ~15);
+    return {row * p.kv_row_bytes, valid ? static_cast<uint32_t>(imin(end - t, 16)) * p.kv_row_bytes : 0u};
+}
+
+// A tile of KT cache tokens of K or V on its way into LDS, by WAVES waves. 16- and
+// 32-bit caches go there directly; FP8 ones through registers (raw), where they
+// are widened when they `land`.
+template <typename QT, int KVF, int D, int WAVES, int KT>
+struct TileLoad {
+    static constexpr bool kWiden = KVF != kTokenNative;
+    static constexpr int ES = kWiden ? 1 : static_cast<int>(sizeof(QT));
+    static constexpr int RB = D * static_cast<int>(sizeof(QT));  // bytes of a row in LDS
+    static constexpr int SB = D * ES;                            // and in the cache
+    static constexpr int RPI = 1024 / SB;                        // rows per request of a wave
+    static constexpr int NL = KT * SB / 1024 / WAVES;            // requests per wave
+    static constexpr int LPR = SB / 16;                          // lanes per row
+    static_assert(NL * WAVES * 1024 == KT * SB && 16 % RPI == 0, "whole requests, within 16 tokens");
+    u32x4 raw[kWiden ? NL : 1];
+
+    // ids: tile_pages of the tile; head: the cache from its KV head on; to: the tile's address in LDS.
+    __device__ __forceinline__ void request(const TokenParams& p, int ids, const char* head, uint32_t to, int t0, int end,
+                                            int wave, int lane) {
+        request_part(std::make_integer_sequence<int, NL>{}, p, ids, head, to + wave * (RPI * RB), t0, end, wave, lane);
     }
-    // Cache tokens that every live row of the tile sees.
-    const int common = token_sees(p.causal, w.context, w.count, w.row0 / p.group);
 
-    const int32_t* pages = p.table + static_cast<int64_t>(w.b) * p.table_width;
-    const char* k_head = static_cast<const char*>(p.k) + static_cast<size_t>(w.kv_head) * D * ES;
-    const char* v_head = static_cast<const char*>(p.v) + static_cast<size_t>(w.kv_head) * D * ES;
+    template <int... kParts>
+    __device__ __forceinline__ void request_part(std::integer_sequence<int, kParts...>, const TokenParams& p, int ids,
+                                                 const char* head, uint32_t to, int t0, int end, int wave, int lane) {
+        (request_one<kParts>(p, ids, head, to, t0, end, wave, lane), ...);
+    }
 
-    // This lane's rows: q as the first product's operand, and what they see.
-    u32x4 q[R][KS];
-    int sees[R];
-    int64_t out_at[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int row = w.row0 + (wave * R + r) * 16 + col;
-        const int token = row / p.group;
-        sees[r] = row < w.rows ? imin(w.end, token_sees(p.causal, w.context, w.count, token)) : 0;
-        out_at[r] = token < p.tokens ? token_q_row(p, w.b, w.kv_head, token, row - token * p.group) * D : -1;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            q[r][s] = u32x4{0, 0, 0, 0};
-            if (row < w.rows)
-                q[r][s] = *reinterpret_cast<const u32x4*>(static_cast<const QT*>(p.q) + out_at[r] + (4 * s + quad) * CE);
+    template <int kPart>
+    __device__ __forceinline__ void request_one(const TokenParams& p, int ids, const char* head, uint32_t to, int t0, int end,
+                                                int wave, int lane) {
+        const int row0 = RPI * (wave + WAVES * kPart);
+        const int block = row0 / 16;
+        const RowBlock rows = row_block(p, __builtin_amdgcn_readlane(ids, block), t0 + 16 * block, end);
+        const int r = row0 % 16 + lane / LPR;
+        if constexpr (kWiden) {
+            const uint32_t offset = r * p.kv_row_bytes + (lane % LPR) * 16;
+            raw[kPart] = __builtin_amdgcn_raw_buffer_load_b128(row_buffer(head + rows.offset, rows.bytes), offset, 0, 0);
+        } else {
+            // LDS slot `lane` of the request holds the chunk that token_chunk puts there.
+            const uint32_t offset = r * p.kv_row_bytes + token_slot_chunk<RB>(r, lane % LPR) * 16;
+            load_to_lds<kPart * WAVES * RPI * RB>(head + rows.offset, rows.bytes, to, offset);
         }
     }
-    f32x4 o[R][ND];
-    float m[R], l[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        m[r] = kNoToken;
-        l[r] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[r][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
 
-    for (int t0 = w.begin; t0 < w.end; t0 += KT) {
-        __syncthreads();
-        // K and V rows of the tile into LDS; rows behind the end and on invalid pages are zeros.
-        for (int i = threadIdx.x; i < KT * CPR; i += WAVES * kWave) {
-            const int r = i / CPR, c = i % CPR;
-            const int t = t0 + r;
-            u32x4 kc = {0, 0, 0, 0}, vc = {0, 0, 0, 0};
-            if (t < w.end) {
-                const int page = pages[t >> p.page_shift];
-                if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.physical_pages)) {
-                    const int64_t row = (static_cast<int64_t>(page) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
-                    const int64_t offset = row * p.kv_row_bytes + c * CE * ES;
-                    if constexpr (KVF == kTokenNative) {
-                        kc = *reinterpret_cast<const u32x4*>(k_head + offset);
-                        vc = *reinterpret_cast<const u32x4*>(v_head + offset);
-                    } else {
-                        const u32x2 kw = *reinterpret_cast<const u32x2*>(k_head + offset);
-                        const u32x2 vw = *reinterpret_cast<const u32x2*>(v_head + offset);
-                        const u32x2 k0 = Math::template widen<KVF>(kw[0]), k1 = Math::template widen<KVF>(kw[1]);
-                        const u32x2 v0 = Math::template widen<KVF>(vw[0]), v1 = Math::template widen<KVF>(vw[1]);
-                        kc = u32x4{k0[0], k0[1], k1[0], k1[1]};
-                        vc = u32x4{v0[0], v0[1], v1[0], v1[1]};
-                    }
+    __device__ __forceinline__ void land(char* tile, int wave, int lane) {
+        if constexpr (kWiden) {
+#pragma unroll
+            for (int jj = 0; jj < NL; ++jj) {
+                const int r = RPI * (wave + WAVES * jj) + lane / LPR;
+                const u32x4 w = raw[jj];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const u32x2 a = TokenMath<QT>::template widen<KVF>(w[2 * half]);
+                    const u32x2 b = TokenMath<QT>::template widen<KVF>(w[2 * half + 1]);
+                    *reinterpret_cast<u32x4*>(tile + token_chunk<RB>(r, 2 * (lane % LPR) + half) * 16) = u32x4{a[0], a[1], b[0], b[1]};
                 }
             }
-            const int at = token_chunk<RB>(r, c) * 16;
-            *reinterpret_cast<u32x4*>(k_tile + at) = kc;
-            *reinterpret_cast<u32x4*>(v_tile + at) = vc;
         }
-        uint32_t invalid = 0;  // blocks of 16 tokens on invalid pages
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int t = t0 + 16 * i;
-            if (t < w.end && static_cast<uint32_t>(pages[t >> p.page_shift]) >= static_cast<uint32_t>(p.physical_pages))
-                invalid |= 1u << i;
-        }
-        __syncthreads();
-        if (t0 + KT > common) {  // uniform
-            bool bad = false;
-            for (int i = threadIdx.x; i < KT * CPR; i += WAVES * kWave)
-                bad |= holds_nonfinite<QT>(*reinterpret_cast<const u32x4*>(v_tile + i * 16));
-            if (__syncthreads_or(bad)) {
-                token_rows_one_by_one<QT, KVF, D, WAVES, M>(p, w, wave, lane);
-                return;
-            }
-        }
+    }
+};
 
-        // Scores, transposed: lane (col, quad) holds row col, tokens 16 i + 4 quad + e.
-        f32x4 s[R][NI];
+// Blocks of 16 tokens of a tile on invalid pages, a bit each.
+template <int KT>
+__device__ __forceinline__ uint32_t invalid_blocks(const TokenParams& p, int ids, int t0, int end, int lane) {
+    const bool bad = static_cast<uint32_t>(ids) >= static_cast<uint32_t>(p.physical_pages) && t0 + 16 * lane < end;
+    return static_cast<uint32_t>(__ballot(bad)) & ((1u << (KT / 16)) - 1);
+}
+
+// A wave's R blocks of 16 rows: q as the first product's operand, what the rows
+// see, and their softmax state.
+template <typename QT, int D, int R>
+struct TokenRowsState {
+    static constexpr bool kF32 = sizeof(QT) == 4;
+    static constexpr int RB = D * static_cast<int>(sizeof(QT));
+    static constexpr int KS = RB / 64;  // steps of four chunks of the first product
+    static constexpr int ND = D / 16;   // blocks of 16 dims of the second
+    using Math = TokenMath<QT>;
+    u32x4 q[R][KS];
+    f32x4 o[R][ND];
+    float m[R], l[R];
+    int sees[R];
+
+    __device__ __forceinline__ void open(const TokenParams& p, const TokenWork& w, int first_row, int lane) {
+        constexpr int CE = 16 / static_cast<int>(sizeof(QT));
+        const int col = lane % 16, quad = lane / 16;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int row = first_row + r * 16 + col;
+            const int token = row / p.group;
+            sees[r] = row < w.rows ? imin(w.end, token_sees(p.causal, w.context, w.count, token)) : 0;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                q[r][s] = u32x4{0, 0, 0, 0};
+                if (row < w.rows)
+                    q[r][s] = *reinterpret_cast<const u32x4*>(static_cast<const QT*>(p.q) +
+                                                              token_q_row(p, w.b, w.kv_head, token, row - token * p.group) * D +
+                                                              (4 * s + quad) * CE);
+            }
+            m[r] = kNoToken;
+            l[r] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[r][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+
+    // Scores of a tile of 16 NI tokens, transposed: lane (col, quad) holds row col, tokens 16 i + 4 quad + e.
+    template <int NI>
+    __device__ __forceinline__ void score(const char* k_tile, f32x4 (&s)[R][NI], int lane) {
+        const int col = lane % 16, quad = lane / 16;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
 #pragma unroll
@@ -328,7 +372,13 @@ __global__ void __launch_bounds__(kWave * WAVES) token_kernel(const TokenParams 
                 }
             }
         }
-        const bool masked = t0 + KT > imin(common, w.end) || invalid != 0 || last - w.row0 != M - 1;  // uniform
+    }
+
+    // Their weights, and the running maximum and sum. t0: the tile's first token; masked (uniform): some row does not see
+    // some token of it.
+    template <int NI>
+    __device__ __forceinline__ void weigh(f32x4 (&s)[R][NI], int t0, bool masked, uint32_t invalid, float scale_log2, int lane) {
+        const int quad = lane / 16;
         float top[R];
         bool grow = false;
 #pragma unroll
@@ -338,8 +388,7 @@ __global__ void __launch_bounds__(kWave * WAVES) token_kernel(const TokenParams 
                 for (int i = 0; i < NI; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int t = t0 + 16 * i + 4 * quad + e;
-                        const bool seen = t < sees[r] && !(invalid >> i & 1u);
+                        const bool seen = t0 + 16 * i + 4 * quad + e < sees[r] && !(invalid >> i & 1u);
                         s[r][i][e] = seen ? s[r][i][e] : -INFINITY;
                     }
             }
@@ -348,7 +397,7 @@ __global__ void __launch_bounds__(kWave * WAVES) token_kernel(const TokenParams 
             for (int i = 0; i < NI; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x = fmaxf(x, s[r][i][e]);
-            top[r] = max_over_lane_groups(x) * p.scale_log2;
+            top[r] = max_over_lane_groups(x) * scale_log2;
             grow |= top[r] > m[r] + Math::kSlack;
         }
         if (__any(grow)) {
@@ -368,11 +417,15 @@ __global__ void __launch_bounds__(kWave * WAVES) token_kernel(const TokenParams 
             for (int i = 0; i < NI; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[r][i][e] = fast_exp2(fmaf(s[r][i][e], p.scale_log2, -m[r]));
+                    s[r][i][e] = fast_exp2(fmaf(s[r][i][e], scale_log2, -m[r]));
                     l[r] += s[r][i][e];
                 }
+    }
 
-        // o^T += V^T w^T, 32 tokens a step (FP32: four).
+    // o^T += V^T w^T, 32 tokens a step (FP32: four).
+    template <int NI>
+    __device__ __forceinline__ void add(const char* v_tile, const f32x4 (&s)[R][NI], int lane) {
+        const int col = lane % 16, quad = lane / 16;
         if constexpr (kF32) {
 #pragma unroll
             for (int i = 0; i < NI; ++i)
@@ -380,9 +433,8 @@ __global__ void __launch_bounds__(kWave * WAVES) token_kernel(const TokenParams 
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int d = 0; d < ND; ++d) {
-                        const int row = 16 * i + 4 * quad + e;
                         const float vf = *reinterpret_cast<const float*>(
-                            v_tile + token_chunk<RB>(row, 4 * d + col / 4) * 16 + (col % 4) * 4);
+                            v_tile + token_chunk<RB>(16 * i + 4 * quad + e, 4 * d + col / 4) * 16 + (col % 4) * 4);
 #pragma unroll
                         for (int r = 0; r < R; ++r)
                             o[r][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, s[r][i][e], o[r][d], 0, 0, 0);
@@ -411,29 +463,267 @@ __global__ void __launch_bounds__(kWave * WAVES) token_kernel(const TokenParams 
             }
         }
     }
+};
 
+// The kernel's arguments, read again: what only the end of a kernel needs would
+// otherwise be held in scalar registers through its loop, which are too few.
+__device__ __forceinline__ TokenParams reloaded_params() {
+    const __attribute__((address_space(4))) TokenParams* p =
+        (const __attribute__((address_space(4))) TokenParams*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const TokenParams*)p;
+}
+
+// The work of a workgroup whose tile has M rows from row0 on; false if no row of it
+// sees a token of its split.
+template <int M>
+__device__ __forceinline__ bool open_work(const TokenParams& p, const TokenCoords& at, TokenWork& w, int& last) {
+    w.b = at.b;
+    w.kv_head = at.kv_head;
+    w.split = at.split;
+    w.row0 = at.tile * M;
+    w.count = token_count(p, w.b);
+    w.context = token_context(p, w.b);
+    w.rows = w.count * p.group;
+    last = imin(w.row0 + M, w.rows) - 1;
+    const int span = token_split(p.splits, p.split_tokens, w.context);
+    w.begin = w.split * span;
+    w.end = last < w.row0 ? 0 : imin(w.begin + span, token_sees(p.causal, w.context, w.count, last / p.group));
+    return w.begin < w.end;
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: a workgroup of WAVES waves, R blocks of 16 rows each, over tiles of
+// KT cache tokens that the waves share through LDS, two of them so that the
+// next is on its way while one is used.
+template <typename QT, int KVF, int D, int R, int WAVES, int KT>
+__global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenParams p) {
+    using Rows = TokenRowsState<QT, D, R>;
+    using Load = TileLoad<QT, KVF, D, WAVES, KT>;
+    constexpr int RB = Rows::RB;
+    constexpr int M = WAVES * R * 16;
+    constexpr int TILE = KT * RB;
+    __shared__ __attribute__((aligned(1024))) char k_tiles[2 * TILE];
+    __shared__ __attribute__((aligned(1024))) char v_tiles[2 * TILE];
+
+    const int lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    TokenWork w;
+    int last;
+    if (!open_work<M>(p, token_coords(p, blockIdx.x), w, last)) {
+        if (p.splits == 1)  // states of such splits are never read
+            for (int i = wave; i < M; i += WAVES) store_row_zeros<QT, D>(p, w, w.row0 + i, lane);
+        return;
+    }
+    // Cache tokens that every live row of the tile sees.
+    const int common = imin(w.end, token_sees(p.causal, w.context, w.count, w.row0 / p.group));
+    const bool partial = last - w.row0 != M - 1;
+    const char* k_head = static_cast<const char*>(p.k) + static_cast<size_t>(w.kv_head) * Load::SB;
+    const char* v_head = static_cast<const char*>(p.v) + static_cast<size_t>(w.kv_head) * Load::SB;
+    const int32_t* pages = p.table + static_cast<int64_t>(w.b) * p.table_width;
+    Load k_load, v_load;
+    int ids = tile_pages<KT>(p, pages, w.begin, lane);
+    uint32_t invalid = invalid_blocks<KT>(p, ids, w.begin, w.end, lane);
+    const uint32_t k_at = lds_address(k_tiles), v_at = lds_address(v_tiles);
+    k_load.request(p, ids, k_head, k_at, w.begin, w.end, wave, lane);
+    v_load.request(p, ids, v_head, v_at, w.begin, w.end, wave, lane);
+    ids = tile_pages<KT>(p, pages, w.begin + KT, lane);
+    Rows rows;
+    rows.open(p, w, w.row0 + wave * R * 16, lane);
+
+    int buffer = 0;
+    for (int t0 = w.begin; t0 < w.end; t0 += KT, buffer ^= 1) {
+        char* k_tile = k_tiles + buffer * TILE;
+        char* v_tile = v_tiles + buffer * TILE;
+        k_load.land(k_tile, wave, lane);
+        v_load.land(v_tile, wave, lane);
+        wait_for_loads();  // this wave's part of the tile is in LDS
+        __syncthreads();   // everyone's part is, and the other tile is no longer read
+        const uint32_t here = invalid;
+        // Behind the end the request has no rows: it writes zeros that nothing reads.
+        invalid = invalid_blocks<KT>(p, ids, t0 + KT, w.end, lane);
+        k_load.request(p, ids, k_head, k_at + (buffer ^ 1) * TILE, t0 + KT, w.end, wave, lane);
+        v_load.request(p, ids, v_head, v_at + (buffer ^ 1) * TILE, t0 + KT, w.end, wave, lane);
+        ids = tile_pages<KT>(p, pages, t0 + 2 * KT, lane);
+        if (t0 + KT > common) {  // uniform
+            bool bad = false;
+            for (int i = threadIdx.x; i < TILE / 16; i += WAVES * kWave)
+                bad |= holds_nonfinite<QT>(*reinterpret_cast<const u32x4*>(v_tile + i * 16));
+            if (__syncthreads_or(bad)) {
+                wait_for_loads();
+                token_rows_one_by_one<QT, KVF, D>(p, w, M, wave, WAVES, lane);
+                return;
+            }
+        }
+        f32x4 s[R][KT / 16];
+        rows.score(k_tile, s, lane);
+        rows.weigh(s, t0, t0 + KT > common || here != 0 || partial, here, p.scale_log2, lane);
+        rows.add(v_tile, s, lane);
+    }
+    wait_for_loads();  // the last request's: nothing may write LDS behind the workgroup's end
+
+    const int col = lane % 16, quad = lane / 16;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const float sum = sum_over_lane_groups(l[r]);
+        const float sum = sum_over_lane_groups(rows.l[r]);
         const int row = w.row0 + (wave * R + r) * 16 + col;
+        const int token = row / p.group;
         if (p.splits == 1) {
-            if (out_at[r] < 0) continue;
+            if (token >= p.tokens) continue;
             const float inv = sum == 0.0f ? 0.0f : p.v_scale / sum;
-            QT* out = static_cast<QT*>(p.out) + out_at[r];
+            QT* out = static_cast<QT*>(p.out) + token_q_row(p, w.b, w.kv_head, token, row - token * p.group) * D;
 #pragma unroll
-            for (int d = 0; d < ND; ++d) {
+            for (int d = 0; d < Rows::ND; ++d) {
                 f32x4 x;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = sum == 0.0f ? 0.0f : o[r][d][e] * inv;
-                if constexpr (kF32) *reinterpret_cast<f32x4*>(out + 16 * d + 4 * quad) = x;
-                else *reinterpret_cast<u32x2*>(out + 16 * d + 4 * quad) = u32x2{Math::pack(x[0], x[1]), Math::pack(x[2], x[3])};
+                for (int e = 0; e < 4; ++e) x[e] = sum == 0.0f ? 0.0f : rows.o[r][d][e] * inv;
+                if constexpr (Rows::kF32) *reinterpret_cast<f32x4*>(out + 16 * d + 4 * quad) = x;
+                else
+                    *reinterpret_cast<u32x2*>(out + 16 * d + 4 * quad) =
+                        u32x2{Rows::Math::pack(x[0], x[1]), Rows::Math::pack(x[2], x[3])};
             }
         } else if (row < w.rows) {
             const int64_t state = token_state(p, w.b, w.kv_head, row, w.split);
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
-                *reinterpret_cast<f32x4*>(p.numerator + state * D + 16 * d + 4 * quad) = o[r][d] * p.v_scale;
-            if (quad == 0) *reinterpret_cast<float2*>(p.stats + state * 2) = make_float2(m[r], sum);
+            for (int d = 0; d < Rows::ND; ++d)
+                *reinterpret_cast<f32x4*>(p.numerator + state * D + 16 * d + 4 * quad) = rows.o[r][d] * p.v_scale;
+            if (quad == 0) *reinterpret_cast<float2*>(p.stats + state * 2) = make_float2(rows.m[r], sum);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: every wave streams cache tokens of its own, tiles of 32 from
+// its part of LDS, for all R blocks of 16 rows, and the workgroup's waves of
+// one KV head combine at the end. The next K is requested once a tile is scored,
+// the next V once it is added, so that a wave always has loads in flight.
+template <typename QT, int KVF, int D, int R, int WAVES>
+struct StreamShape {
+    static constexpr int KT = 32;
+    static constexpr int RB = D * static_cast<int>(sizeof(QT));
+    static constexpr int TILE = KT * RB;
+    static constexpr int SD = D + 4;  // floats from one row's sums to the next: rows begin in other banks
+    static constexpr int STATE = R * 16 * SD * 4;
+    static constexpr int REGION = 2 * TILE > STATE ? 2 * TILE : STATE;
+};
+
+template <typename QT, int KVF, int D, int R, int WAVES>
+__global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const TokenParams p) {
+    using Rows = TokenRowsState<QT, D, R>;
+    using Shape = StreamShape<QT, KVF, D, R, WAVES>;
+    constexpr int KT = Shape::KT;
+    using Load = TileLoad<QT, KVF, D, 1, KT>;
+    constexpr int M = R * 16;
+    __shared__ __attribute__((aligned(1024))) char regions[WAVES * Shape::REGION];
+    __shared__ float2 states[WAVES][M];
+
+    const int lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const TokenCoords at = token_stream_coords(p, blockIdx.x, wave);
+    const int slice = wave / p.head_waves, slices = WAVES / p.head_waves;
+    TokenWork w;
+    int last;
+    if (!open_work<M>(p, at, w, last)) {  // the same for all waves
+        if (p.splits == 1)
+            for (int i = slice; i < M; i += slices) store_row_zeros<QT, D>(p, w, w.row0 + i, lane);
+        return;
+    }
+    const int common = imin(w.end, token_sees(p.causal, w.context, w.count, w.row0 / p.group));
+    const bool partial = last - w.row0 != M - 1;
+    const char* k_head = static_cast<const char*>(p.k) + static_cast<size_t>(w.kv_head) * Load::SB;
+    const char* v_head = static_cast<const char*>(p.v) + static_cast<size_t>(w.kv_head) * Load::SB;
+    const int32_t* pages = p.table + static_cast<int64_t>(w.b) * p.table_width;
+    char* k_tile = regions + wave * Shape::REGION;
+    char* v_tile = k_tile + Shape::TILE;
+    const uint32_t k_at = lds_address(regions) + wave * Shape::REGION, v_at = k_at + Shape::TILE;
+    const int step = slices * KT;
+    const int first = w.begin + slice * KT;
+
+    Load k_load, v_load;
+    int ids = tile_pages<KT>(p, pages, first, lane);
+    int next_ids = tile_pages<KT>(p, pages, first + step, lane);
+    k_load.request(p, ids, k_head, k_at, first, w.end, 0, lane);
+    v_load.request(p, ids, v_head, v_at, first, w.end, 0, lane);
+    Rows rows;
+    rows.open(p, w, w.row0, lane);
+    bool bad = false;
+    for (int t0 = first; t0 < w.end; t0 += step) {
+        const uint32_t invalid = invalid_blocks<KT>(p, ids, t0, w.end, lane);
+        const bool masked = t0 + KT > common || invalid != 0 || partial;
+        f32x4 s[R][KT / 16];
+        // Requests behind the end have no rows: they write zeros that nothing reads, and keep the counts the same.
+        if constexpr (!Load::kWiden) wait_for_loads<Load::NL>();  // all but V's
+        k_load.land(k_tile, 0, lane);
+        const int later_ids = tile_pages<KT>(p, pages, t0 + 2 * step, lane);
+        if constexpr (Load::kWiden) k_load.request(p, next_ids, k_head, k_at, t0 + step, w.end, 0, lane);
+        rows.score(k_tile, s, lane);
+        if constexpr (!Load::kWiden) {
+            wait_for_reads();
+            k_load.request(p, next_ids, k_head, k_at, t0 + step, w.end, 0, lane);
+        }
+        rows.weigh(s, t0, masked, invalid, p.scale_log2, lane);
+        if constexpr (!Load::kWiden) wait_for_loads<Load::NL>();  // all but the next K's
+        v_load.land(v_tile, 0, lane);
+        if constexpr (Load::kWiden) v_load.request(p, next_ids, v_head, v_at, t0 + step, w.end, 0, lane);
+        if (t0 + KT > common) {
+            for (int i = lane; i < Shape::TILE / 16; i += kWave)
+                bad |= holds_nonfinite<QT>(*reinterpret_cast<const u32x4*>(v_tile + i * 16));
+            if (__any(bad)) break;
+        }
+        rows.add(v_tile, s, lane);
+        if constexpr (!Load::kWiden) {
+            wait_for_reads();
+            v_load.request(p, next_ids, v_head, v_at, t0 + step, w.end, 0, lane);
+        }
+        ids = next_ids;
+        next_ids = later_ids;
+    }
+    wait_for_loads();
+    const TokenParams late = reloaded_params();
+    if (__syncthreads_or(bad)) {
+        token_rows_one_by_one<QT, KVF, D>(late, w, M, slice, slices, lane);
+        return;
+    }
+
+    // The waves' states, into their own parts of LDS.
+    float* sums = reinterpret_cast<float*>(k_tile);
+    const int col = lane % 16, quad = lane / 16;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float sum = sum_over_lane_groups(rows.l[r]);
+#pragma unroll
+        for (int d = 0; d < Rows::ND; ++d)
+            *reinterpret_cast<f32x4*>(sums + (r * 16 + col) * Shape::SD + 16 * d + 4 * quad) = rows.o[r][d];
+        if (quad == 0) states[wave][r * 16 + col] = make_float2(rows.m[r], sum);
+    }
+    __syncthreads();
+    constexpr int PER = D / kWave;
+    for (int i = slice; i < M; i += slices) {
+        const int row = w.row0 + i, token = row / late.group;
+        if (token >= late.tokens) break;
+        float m = kNoToken, l = 0.0f, o[PER];
+        for (int j = wave % late.head_waves; j < WAVES; j += late.head_waves)
+            if (states[j][i].y != 0.0f) m = fmaxf(m, states[j][i].x);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) o[e] = 0.0f;
+        for (int j = wave % late.head_waves; j < WAVES; j += late.head_waves) {
+            const float2 st = states[j][i];
+            const float a = st.y != 0.0f ? fast_exp2(st.x - m) : 0.0f;
+            l += st.y * a;
+            const float* from = reinterpret_cast<const float*>(regions + j * Shape::REGION) + i * Shape::SD + lane * PER;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) o[e] = fmaf(from[e], a, o[e]);
+        }
+        if (late.splits == 1) {
+            QT* out = static_cast<QT*>(late.out) + token_q_row(late, w.b, w.kv_head, token, row - token * late.group) * D + lane * PER;
+            const float inv = l == 0.0f ? 0.0f : late.v_scale / l;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) out[e] = static_cast<QT>(l == 0.0f ? 0.0f : o[e] * inv);
+        } else if (row < w.rows) {
+            const int64_t state = token_state(late, w.b, w.kv_head, row, w.split);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) late.numerator[state * D + lane * PER + e] = o[e] * late.v_scale;
+            if (lane == 0) *reinterpret_cast<float2*>(late.stats + state * 2) = make_float2(m, l);
         }
     }
 }

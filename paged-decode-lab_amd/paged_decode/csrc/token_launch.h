@@ -15,9 +15,20 @@ int launch_tokens_bf16_d128(const TokenParams&, const TokenPlan&, int kv_dtype, 
 
 template <typename QT, int KVF, int D>
 int launch_tokens_format(const TokenParams& p, const TokenPlan& plan, hipStream_t stream) {
+    const dim3 grid(static_cast<uint32_t>(plan.workgroups));
     constexpr int KT = sizeof(QT) == 4 ? 32 : 64;
-    hipLaunchKernelGGL((token_kernel<QT, KVF, D, 1, 4, KT>), dim3(static_cast<uint32_t>(plan.workgroups)), dim3(4 * kWave), 0,
-                       stream, p);
+    if (plan.stream) {
+        constexpr int WAVES = sizeof(QT) == 4 && D == 128 ? kStreamWaves / 2 : kStreamWaves;
+        if (plan.tile_rows == 16) {
+            hipLaunchKernelGGL((token_stream_kernel<QT, KVF, D, 1, WAVES>), grid, dim3(WAVES * kWave), 0, stream, p);
+        } else {
+            hipLaunchKernelGGL((token_stream_kernel<QT, KVF, D, 2, WAVES>), grid, dim3(WAVES * kWave), 0, stream, p);
+        }
+    } else if (plan.tile_rows == 64) {
+        hipLaunchKernelGGL((token_kernel<QT, KVF, D, 1, 4, KT>), grid, dim3(4 * kWave), 0, stream, p);
+    } else if constexpr (!(sizeof(QT) == 4 && D == 128)) {
+        hipLaunchKernelGGL((token_kernel<QT, KVF, D, 2, 4, KT>), grid, dim3(4 * kWave), 0, stream, p);
+    }
     if (p.splits > 1) {
         const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens * p.query_heads;
         hipLaunchKernelGGL((token_merge_kernel<QT, D>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream, p);

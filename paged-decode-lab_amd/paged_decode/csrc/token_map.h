@@ -32,6 +32,7 @@ struct TokenParams {
     int splits;              // of each sequence's cache tokens
     int split_tokens;        // tokens per split where `splits` of them reach the length
     int tile_rows, row_tiles;
+    int head_waves;          // stream kernel: KV heads of a workgroup
     uint32_t kv_row_bytes;   // bytes from one cache token to the next: kv_heads * D * element
     float scale_log2;        // k_scale / sqrt(D) * log2(e)
     float v_scale;
@@ -78,6 +79,20 @@ PD_HD TokenCoords token_coords(const TokenParams& p, uint32_t block) {
     return c;
 }
 
+// Stream kernel: workgroups of one split's KV heads are neighbours, wave w has
+// KV head w % head_waves of the workgroup's.
+PD_HD TokenCoords token_stream_coords(const TokenParams& p, uint32_t block, int wave) {
+    const uint32_t head_groups = static_cast<uint32_t>(p.kv_heads / p.head_waves);
+    const uint32_t unit = block / head_groups;
+    const uint32_t part = unit / p.row_tiles;
+    TokenCoords c;
+    c.kv_head = static_cast<int>(block - unit * head_groups) * p.head_waves + wave % p.head_waves;
+    c.tile = static_cast<int>(unit - part * p.row_tiles);
+    c.b = static_cast<int>(part / p.splits);
+    c.split = static_cast<int>(part - static_cast<uint32_t>(c.b) * p.splits);
+    return c;
+}
+
 // State of row `row` (of the padded rows of all tiles) of (sequence, KV head) in split s.
 PD_HD int64_t token_state(const TokenParams& p, int b, int kv_head, int row, int s) {
     const int64_t rows = static_cast<int64_t>(p.row_tiles) * p.tile_rows;
@@ -99,11 +114,20 @@ PD_HD int token_chunk(int r, int c) {
     return r * 32 + (c ^ (r & 15));                                                          // FP32, D 128
 }
 
+// The chunk of row r that lies at position `slot` of the row's chunks: the
+// permutation is its own inverse.
+template <int kRowBytes>
+PD_HD int token_slot_chunk(int r, int slot) {
+    return token_chunk<kRowBytes>(r, slot) - r * (kRowBytes / 16);
+}
+
 // ---------------------------------------------------------------------------
 // Launch planning (host).
 
 struct TokenPlan {
+    bool stream;             // the kernel of few rows
     int tile_rows, row_tiles;
+    int waves, head_waves;   // of a workgroup; stream kernel: KV heads among them
     int splits, split_tokens;
     int64_t workgroups;
     int64_t states;  // 0 with one split
@@ -111,16 +135,29 @@ struct TokenPlan {
 
 constexpr int kTokenMinSplit = 256;    // cache tokens per split, at least
 constexpr int kTokenGroupsPerCu = 2;   // workgroups per CU that a split aims at
+constexpr int kStreamMaxRows = 32;     // rows that the stream kernel takes
+constexpr int kStreamWaves = 8;        // waves of its workgroups (FP32 rows are twice as long: 4)
 
-inline TokenPlan plan_tokens(int batch, int tokens, int query_heads, int kv_heads, int64_t bound, int64_t max_states,
-                             int compute_units) {
+// q_bytes: of a q element. bound: cache tokens the host knows no sequence to exceed.
+inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads, int64_t bound,
+                             int64_t max_states, int compute_units) {
     TokenPlan t{};
     const int64_t rows = static_cast<int64_t>(tokens) * (query_heads / kv_heads);
-    t.tile_rows = 64;
+    t.stream = rows <= kStreamMaxRows;
+    if (t.stream) {
+        t.tile_rows = rows <= 16 ? 16 : 32;
+        t.waves = q_bytes == 4 && head_dim == 128 ? kStreamWaves / 2 : kStreamWaves;
+        t.head_waves = kv_heads % 2 == 0 ? 2 : 1;
+    } else {
+        t.tile_rows = rows <= 64 || (q_bytes == 4 && head_dim == 128) ? 64 : 128;
+        t.waves = 4;
+        t.head_waves = 1;
+    }
     t.row_tiles = static_cast<int>((rows + t.tile_rows - 1) / t.tile_rows);
     const int64_t units = static_cast<int64_t>(batch) * kv_heads * t.row_tiles;
-    const int64_t wanted = static_cast<int64_t>(compute_units) * kTokenGroupsPerCu;
-    int64_t splits = units < wanted ? (wanted + units - 1) / units : 1;
+    const int64_t groups = units / t.head_waves;
+    const int64_t wanted = static_cast<int64_t>(compute_units) * (t.stream ? 1 : kTokenGroupsPerCu);
+    int64_t splits = groups < wanted ? (wanted + groups - 1) / groups : 1;
     splits = lmin(splits, lmin((bound + kTokenMinSplit - 1) / kTokenMinSplit, max_states / (units * t.tile_rows)));
     t.splits = 1;
     t.split_tokens = kTokenSplitUnit;
@@ -129,9 +166,25 @@ inline TokenPlan plan_tokens(int batch, int tokens, int query_heads, int kv_head
         t.split_tokens = static_cast<int>((even + kTokenSplitUnit - 1) / kTokenSplitUnit * kTokenSplitUnit);
         t.splits = static_cast<int>((bound + t.split_tokens - 1) / t.split_tokens);
     }
-    t.workgroups = units * t.splits;
+    t.workgroups = groups * t.splits;
     t.states = t.splits > 1 ? units * t.tile_rows * t.splits : 0;
     return t;
+}
+
+// States with which no call of up to `tokens` tokens splits less than it would with more.
+inline int64_t most_token_states(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads, int64_t reach,
+                                 int compute_units) {
+    int64_t states = 0;
+    for (int n = 1; n <= tokens; ++n) {
+        const TokenPlan t = plan_tokens(q_bytes, head_dim, batch, n, query_heads, kv_heads, reach, INT64_MAX, compute_units);
+        const int64_t units = t.workgroups / t.splits * t.head_waves;
+        const int64_t wanted = static_cast<int64_t>(compute_units) * (t.stream ? 1 : kTokenGroupsPerCu) * t.head_waves;
+        if (units >= wanted && !t.stream) break;  // and so for every larger n
+        // A shorter context takes at most these splits, rounded to whole units of tokens.
+        const int64_t most = lmin((wanted + units - 1) / units, (reach + kTokenMinSplit - 1) / kTokenMinSplit);
+        if (most > 1 && most * units * t.tile_rows > states) states = most * units * t.tile_rows;
+    }
+    return states;
 }
 
 }  // namespace pd

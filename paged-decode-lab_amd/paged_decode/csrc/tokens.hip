@@ -49,16 +49,8 @@ size_t pd_decode_tokens_workspace(int q_dtype, int kv_dtype, int batch, int toke
         return 0;
     const int cus = compute_units > 0 ? compute_units : device_cus();
     const int64_t reach = static_cast<int64_t>(table_width) * page_size;
-    int64_t states = 0;
-    for (int n = 1; n <= tokens; ++n) {
-        // The splits of a context grow with it, but for the rounding of their length: every multiple of it counts.
-        const TokenPlan t = plan_tokens(batch, n, query_heads, kv_heads, reach, INT64_MAX, cus);
-        const int64_t units = t.workgroups / t.splits;
-        const int64_t wanted = static_cast<int64_t>(cus) * kTokenGroupsPerCu;
-        if (units >= wanted) break;  // and so for every larger n
-        const int64_t most = lmin((wanted + units - 1) / units, (reach + kTokenMinSplit - 1) / kTokenMinSplit);
-        if (most > 1 && most * units * t.tile_rows > states) states = most * units * t.tile_rows;
-    }
+    const int64_t states = most_token_states(q_dtype == PD_DTYPE_F32 ? 4 : 2, head_dim, batch, tokens, query_heads, kv_heads,
+                                             reach, cus);
     return static_cast<size_t>(states) * state_bytes(head_dim);
 }
 
@@ -85,7 +77,8 @@ int pd_decode_tokens(const void* q, int q_dtype, const void* k, const void* v, i
         bound = std::min(std::max<int64_t>(bound, 1), reach);
     }
     const int64_t max_states = static_cast<int64_t>(workspace_bytes / state_bytes(head_dim));
-    const TokenPlan plan = plan_tokens(batch, tokens, query_heads, kv_heads, bound, max_states, device_cus());
+    const TokenPlan plan = plan_tokens(q_dtype == PD_DTYPE_F32 ? 4 : 2, head_dim, batch, tokens, query_heads, kv_heads, bound,
+                                       max_states, device_cus());
     if (plan.workgroups > 0x7FFFFFFF || static_cast<int64_t>(batch) * tokens * query_heads > 0x7FFFFFFFLL * 4) return PD_ERR_SHAPE;
 
     TokenParams p{};
@@ -111,6 +104,7 @@ int pd_decode_tokens(const void* q, int q_dtype, const void* k, const void* v, i
     p.split_tokens = plan.split_tokens;
     p.tile_rows = plan.tile_rows;
     p.row_tiles = plan.row_tiles;
+    p.head_waves = plan.head_waves;
     const int element = kv_dtype == PD_DTYPE_F32 ? 4 : kv_dtype == PD_DTYPE_F16 || kv_dtype == PD_DTYPE_BF16 ? 2 : 1;
     p.kv_row_bytes = static_cast<uint32_t>(kv_heads) * head_dim * element;
     p.scale_log2 = static_cast<float>(static_cast<double>(k_scale) / std::sqrt(static_cast<double>(head_dim)) * 1.4426950408889634);
