@@ -23,26 +23,40 @@ constexpr int kAdvanceWaves = 8;        // and of one that holds a whole sequenc
 constexpr int kMaxPairs = 64;           // rotated pairs of a head
 constexpr double kTurnsPerRadian = 0.15915494309189533576888;
 
+// Eight stored values as they are read, and as FP32.
 template <typename T>
 struct Eight {
-    T x[8];
+    u32x4 w;
+    __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const u32x4*>(p); }
+    __device__ __forceinline__ void widen(float (&f)[8]) const {
+        typedef T Vec __attribute__((ext_vector_type(8)));
+        const Vec v = __builtin_bit_cast(Vec, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = static_cast<float>(v[e]);
+    }
 };
 
-__device__ __forceinline__ void load_eight(const float* p, float (&f)[8]) {
-    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        f[e] = a[e];
-        f[4 + e] = b[e];
+template <>
+struct Eight<float> {
+    f32x4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = reinterpret_cast<const f32x4*>(p)[0];
+        b = reinterpret_cast<const f32x4*>(p)[1];
     }
-}
+    __device__ __forceinline__ void widen(float (&f)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f[e] = a[e];
+            f[4 + e] = b[e];
+        }
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ void load_eight(const T* p, float (&f)[8]) {
-    typedef T Vec __attribute__((ext_vector_type(8)));
-    const Vec v = *reinterpret_cast<const Vec*>(p);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = static_cast<float>(v[e]);
+    Eight<T> x;
+    x.load(p);
+    x.widen(f);
 }
 
 __device__ __forceinline__ void store_eight(float* p, const float (&f)[8]) {
@@ -119,16 +133,42 @@ __device__ __forceinline__ bool sequence_fits(const AppendParams& a, const int32
     return __all(fits);
 }
 
+// What a lane holds of one head group of a token: which head, and its dims as stored.
+template <typename T>
+struct LaneHead {
+    int kind;  // 0 q, 1 k, 2 v, -1 no head
+    int h;
+    Eight<T> x, y;
+};
+
+template <typename T, int D>
+__device__ __forceinline__ LaneHead<T> load_head(const RotateParams& p, int b, int token, bool live, int group, int lane, ChunkPair ch) {
+    constexpr int LPH = D / kRotateLaneDims;
+    LaneHead<T> r;
+    const int head = group * (kWave / LPH) + lane / LPH;
+    r.kind = head < p.q_heads ? 0 : head < p.q_heads + p.kv_heads ? 1 : head < p.heads ? 2 : -1;
+    r.h = r.kind == 0 ? head : r.kind == 1 ? head - p.q_heads : head - p.q_heads - p.kv_heads;
+    if (live && r.kind >= 0) {
+        const TokenRows& rows = r.kind == 0 ? p.q : r.kind == 1 ? p.k : p.v;
+        const T* in = reinterpret_cast<const T*>(rows.data) + token_row_offset(rows, b, token, r.h, D);
+        r.x.load(in + ch.first);
+        r.y.load(in + ch.second);
+    }
+    return r;
+}
+
 // One wave's head groups [group0, group0 + groups) of token `token` of sequence b at
-// position pos; turns: the wave's (cos, sin) pairs in LDS.
+// position pos; turns: the wave's (cos, sin) pairs in LDS. A group's heads
+// are requested before the one in front is worked on (the first before the angles).
 template <typename T, int CF, int D>
 __device__ __forceinline__ void rotate_token(const RotateParams& p, int b, int token, int64_t pos, bool live, int64_t cache_row,
                                              int group0, int groups, int lane, float2* turns) {
     constexpr int LPH = D / kRotateLaneDims;  // lanes per head
-    constexpr int HPW = kWave / LPH;          // heads per wave
     const int j = lane % LPH;
     const ChunkPair ch = rotate_chunks(p.rotary_dim, p.interleaved, j);
     const bool turned = j < p.rotary_dim / kRotateLaneDims;
+    LaneHead<T> next = load_head<T, D>(p, b, token, live, group0, lane, ch);
+    float cs[8], sn[8];
     if (p.rotary_dim > 0) {
         if (lane < p.rotary_dim / 2) {
             const float2 t = turn_cos_sin(static_cast<double>(pos) * (p.frequencies[lane] * kTurnsPerRadian));
@@ -136,7 +176,6 @@ __device__ __forceinline__ void rotate_token(const RotateParams& p, int b, int t
         }
         __builtin_amdgcn_wave_barrier();
     }
-    float cs[8], sn[8];
     if (turned) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -147,11 +186,11 @@ __device__ __forceinline__ void rotate_token(const RotateParams& p, int b, int t
     }
     const int64_t out_token = static_cast<int64_t>(b) * p.tokens + token;
     for (int g = group0; g < group0 + groups; ++g) {
-        const int head = g * HPW + lane / LPH;
-        if (head >= p.heads) continue;
-        const bool is_q = head < p.q_heads;
-        const bool is_k = !is_q && head < p.q_heads + p.kv_heads;
-        const int h = is_q ? head : is_k ? head - p.q_heads : head - p.q_heads - p.kv_heads;
+        const LaneHead<T> head = next;
+        if (g + 1 < group0 + groups) next = load_head<T, D>(p, b, token, live, g + 1, lane, ch);
+        const bool is_q = head.kind == 0, is_k = head.kind == 1;
+        const int h = head.h;
+        if (head.kind < 0) continue;
         if (!live) {  // rows behind a sequence's tokens: zeros in q, the cache as it was
             if (is_q) {
                 T* out = reinterpret_cast<T*>(p.q_out) + (out_token * p.q_heads + h) * D;
@@ -161,11 +200,9 @@ __device__ __forceinline__ void rotate_token(const RotateParams& p, int b, int t
             }
             continue;
         }
-        const TokenRows& rows = is_q ? p.q : is_k ? p.k : p.v;
-        const T* in = reinterpret_cast<const T*>(rows.data) + token_row_offset(rows, b, token, h, D);
         float x[8], y[8];
-        load_eight(in + ch.first, x);
-        load_eight(in + ch.second, y);
+        head.x.widen(x);
+        head.y.widen(y);
         const void* weight = is_q ? p.q_weight : is_k ? p.k_weight : nullptr;
         if (weight != nullptr) {
             float sum = 0.0f;

@@ -728,17 +728,22 @@ __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const Token
     }
 }
 
-// Splits of each row into its output: a wave per row.
+// ---------------------------------------------------------------------------
+// Splits of each row into its output: a wave per row, four dims a lane, so that
+// kWave / (D / 4) states are read at once, kUnroll times over before the first is used:
+// a row's reads are what the kernel waits for.
 template <typename QT, int D>
 __global__ void __launch_bounds__(256) token_merge_kernel(const TokenParams p) {
-    constexpr int PER = D / kWave;
+    constexpr int LPS = D / 4;          // lanes per state
+    constexpr int SPW = kWave / LPS;    // states per read
+    constexpr int kUnroll = 4;
     const int lane = threadIdx.x % kWave;
     const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
     const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens * p.query_heads;
     if (item >= rows) return;
-    const int head = static_cast<int>(item % p.query_heads);
-    const int64_t bt = item / p.query_heads;
-    const int b = static_cast<int>(bt / p.tokens), token = static_cast<int>(bt % p.tokens);
+    const uint32_t bt = static_cast<uint32_t>(item / p.query_heads);
+    const int head = static_cast<int>(item - static_cast<int64_t>(bt) * p.query_heads);
+    const int b = static_cast<int>(bt / p.tokens), token = static_cast<int>(bt - static_cast<uint32_t>(b) * p.tokens);
     const int kv_head = head / p.group;
     const int count = token_count(p, b), context = token_context(p, b);
     const int sees = token < count ? token_sees(p.causal, context, count, token) : 0;
@@ -746,25 +751,52 @@ __global__ void __launch_bounds__(256) token_merge_kernel(const TokenParams p) {
     const int live = (sees + span - 1) / span;  // splits that hold a token it sees
     const int64_t state = token_state(p, b, kv_head, token * p.group + head - kv_head * p.group, 0);
     const float2* stats = reinterpret_cast<const float2*>(p.stats) + state;
+    const float* numerator = p.numerator + state * D;
+
     float m = kNoToken;
-    for (int s = 0; s < live; ++s) {
-        const float2 st = stats[s];
-        m = st.y != 0.0f ? fmaxf(m, st.x) : m;
+    for (int s0 = 0; s0 < live; s0 += kWave) {
+        const float2 st = stats[imin(s0 + lane, live - 1)];
+        m = fmaxf(m, st.y != 0.0f ? st.x : kNoToken);
     }
-    float l = 0.0f, o[PER];
+    m = wave_max(m);
+    float l = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0; s0 < live; s0 += kWave) {
+        const float2 st = stats[imin(s0 + lane, live - 1)];
+        const float a = s0 + lane < live && st.y != 0.0f ? fast_exp2(st.x - m) : 0.0f;
+        l += a != 0.0f ? st.y * a : 0.0f;
+        const int here = imin(live - s0, kWave);
+        for (int s = 0; s < here; s += SPW * kUnroll) {
+            f32x4 x[kUnroll];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) o[e] = 0.0f;
-    for (int s = 0; s < live; ++s) {
-        const float2 st = stats[s];
-        if (st.y == 0.0f) continue;
-        const float a = fast_exp2(st.x - m);
-        l += st.y * a;
+            for (int u = 0; u < kUnroll; ++u) {
+                const int at = imin(s0 + s + u * SPW + lane / LPS, live - 1);
+                x[u] = *reinterpret_cast<const f32x4*>(numerator + static_cast<int64_t>(at) * D + (lane % LPS) * 4);
+            }
 #pragma unroll
-        for (int e = 0; e < PER; ++e) o[e] = fmaf(p.numerator[(state + s) * D + lane * PER + e], a, o[e]);
+            for (int u = 0; u < kUnroll; ++u) {
+                const int from = s + u * SPW + lane / LPS;
+                const float weight = __shfl(a, from & (kWave - 1));
+                // A state of weight 0 (none at all, or one with nothing in it) adds nothing, whatever it holds.
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = from < here && weight != 0.0f ? fmaf(x[u][e], weight, o[e]) : o[e];
+            }
+        }
     }
-    QT* out = static_cast<QT*>(p.out) + item * D + lane * PER;
+    l = wave_sum(l);
 #pragma unroll
-    for (int e = 0; e < PER; ++e) out[e] = static_cast<QT>(l == 0.0f ? 0.0f : o[e] / l);
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (LPS == 16) o[e] += __shfl_xor(o[e], 16);
+        o[e] += __shfl_xor(o[e], 32);
+    }
+    if (lane < LPS) {
+        QT* out = static_cast<QT*>(p.out) + item * D + lane * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = l == 0.0f ? 0.0f : o[e] / l;
+        if constexpr (sizeof(QT) == 4) *reinterpret_cast<f32x4*>(out) = o;
+        else
+            *reinterpret_cast<u32x2*>(out) = u32x2{TokenMath<QT>::pack(o[0], o[1]), TokenMath<QT>::pack(o[2], o[3])};
+    }
 }
 
 }  // namespace pd

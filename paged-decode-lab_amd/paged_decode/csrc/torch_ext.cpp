@@ -19,6 +19,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <string>
 
@@ -379,42 +380,89 @@ void stream_read(torch::Tensor a, torch::Tensor b, int64_t a_bytes, int64_t b_by
                                 static_cast<uint32_t*>(sink.data_ptr()), current_stream(a)));
 }
 
-// A rotation and its norm weights, from the optional tensors of a call.
-pd_rotation rotation_of(const c10::optional<torch::Tensor>& frequencies, int64_t style, double scale,
-                        const c10::optional<torch::Tensor>& q_weight, const c10::optional<torch::Tensor>& k_weight,
-                        double eps, const torch::Tensor& like) {
+// ---------------------------------------------------------------------------
+// Head norms, rotation, rotated appends and the attention of several tokens.
+// Their checks are made here rather than in Python, where they would take longer
+// than the kernels of a decode step; they raise what Python's would.
+#define PD_VALUE(cond, text)                       \
+    do {                                           \
+        if (!(cond)) throw py::value_error(text);  \
+    } while (0)
+#define PD_TYPE(cond, text)                       \
+    do {                                          \
+        if (!(cond)) throw py::type_error(text);  \
+    } while (0)
+
+using OptTensor = c10::optional<torch::Tensor>;
+
+const torch::Tensor* pointer(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }
+
+bool token_type(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
+
+// New tokens' heads: [B, H, D] (one token) or [B, n, H, D].
+struct Rows {
+    int64_t batch, tokens, heads, dim;
+    pd_token_rows rows;
+};
+
+Rows rows_of(const torch::Tensor& t, const torch::Tensor& like, const char* name) {
+    const std::string who(name);
+    const int64_t dims = t.dim();
+    PD_VALUE((dims == 3 || dims == 4) && t.numel() > 0, who + " must be [B, H, D] or [B, tokens, H, D], none of them 0");
+    Rows r{t.size(0), dims == 4 ? t.size(1) : 1, t.size(dims - 2), t.size(dims - 1), {}};
+    PD_VALUE(r.batch <= 65535 && r.tokens <= 65535 && r.heads <= 65535, who + " exceeds 65535 sequences, tokens or heads");
+    PD_VALUE(r.dim == 64 || r.dim == 128, "head_dim must be 64 or 128");
+    PD_TYPE(token_type(t.scalar_type()) && t.scalar_type() == like.scalar_type(),
+            "queries, keys and values must share float32, float16 or bfloat16");
+    PD_VALUE(t.is_cuda() && t.device() == like.device(), "inputs must be on one GPU");
+    PD_VALUE(!t.requires_grad(), "inference only: detach tensors requiring gradients");
+    const int64_t unit = 16 / t.element_size();
+    r.rows = {t.data_ptr(), r.batch > 1 ? t.stride(0) : 0, dims == 4 && r.tokens > 1 ? t.stride(1) : 0};
+    PD_VALUE(t.stride(dims - 1) == 1 && (r.heads == 1 || t.stride(dims - 2) == r.dim) &&
+                 reinterpret_cast<uintptr_t>(r.rows.data) % 16 == 0 && r.rows.batch_stride % unit == 0 &&
+                 r.rows.token_stride % unit == 0,
+             who + " must have contiguous heads, and tokens and sequences apart by multiples of 16 bytes");
+    return r;
+}
+
+// A rotation (frequencies, or none) and the norm weights of a call.
+pd_rotation rotation_of(const OptTensor& frequencies, int64_t style, double scale, const OptTensor& q_weight,
+                        const OptTensor& k_weight, double eps, const Rows* q, const Rows* k, const torch::Tensor& like,
+                        int64_t dim) {
     pd_rotation r{};
     r.style = static_cast<int>(style);
     r.scale = static_cast<float>(scale);
     r.eps = static_cast<float>(eps);
     r.weight_dtype = dtype_code(like);
+    PD_VALUE(frequencies.has_value() || q_weight.has_value() || k_weight.has_value(),
+             "nothing to do: neither a rotation nor norm weights");
+    PD_VALUE(eps >= 0 && std::isfinite(r.eps), "eps must be finite and not negative");
     if (frequencies.has_value()) {
         const auto& f = *frequencies;
-        TORCH_CHECK(f.device() == like.device() && f.is_contiguous() && f.scalar_type() == at::kDouble && f.dim() == 1,
-                    "frequencies must be a contiguous float64 tensor on the inputs' device");
+        PD_VALUE(f.device() == like.device(), "the rotation lives on another device");
+        PD_VALUE(f.scalar_type() == at::kDouble && f.is_contiguous() && f.dim() == 1, "frequencies must be float64 [pairs]");
+        PD_VALUE(2 * f.numel() <= dim, "the rotation turns more dims than a head has");
         r.frequencies = f.data_ptr<double>();
         r.rotary_dim = static_cast<int>(2 * f.numel());
     }
+    if (q_weight.has_value() && k_weight.has_value())
+        PD_TYPE(q_weight->scalar_type() == k_weight->scalar_type(), "norm weights must share the inputs' dtype or float32");
     for (const auto* w : {&q_weight, &k_weight}) {
         if (!w->has_value()) continue;
         const auto& t = **w;
-        TORCH_CHECK(t.device() == like.device() && t.is_contiguous() && (t.dim() == 1 || t.dim() == 2) &&
-                        t.size(-1) == like.size(3) && dtype_code(t) >= 0 && dtype_code(t) <= PD_DTYPE_BF16,
-                    "norm weights must be contiguous [D] or [H, D] tensors on the inputs' device");
+        const Rows* rows = w == &q_weight ? q : k;
+        PD_TYPE(t.scalar_type() == like.scalar_type() || t.scalar_type() == at::kFloat,
+                "norm weights must share the inputs' dtype or float32");
+        PD_VALUE(rows != nullptr && ((t.dim() == 1 && t.size(0) == dim) || (t.dim() == 2 && t.size(0) == rows->heads && t.size(1) == dim)),
+                 "norm weights must be [D] or [H, D], for heads that are given");
+        PD_VALUE(t.device() == like.device() && t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+                 "norm weights must be contiguous, 16-byte aligned, on the inputs' device");
+        PD_VALUE(!t.requires_grad(), "inference only: detach tensors requiring gradients");
         r.weight_dtype = dtype_code(t);
         (w == &q_weight ? r.q_weight : r.k_weight) = t.data_ptr();
         (w == &q_weight ? r.q_weight_per_head : r.k_weight_per_head) = t.dim() == 2;
     }
     return r;
-}
-
-// Strided rows [B, n, H, D]; a dim of one element has no stride of its own.
-pd_token_rows rows_of(const torch::Tensor& t, const torch::Tensor& like) {
-    TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.dim() == 4 && t.scalar_type() == like.scalar_type() &&
-                    t.size(0) == like.size(0) && t.size(1) == like.size(1) && t.size(3) == like.size(3) &&
-                    t.stride(3) == 1 && (t.size(2) == 1 || t.stride(2) == t.size(3)),
-                "expected rows [B, tokens, heads, D] of one dtype with contiguous heads on one GPU");
-    return {t.data_ptr(), t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0};
 }
 
 // Whether the memory of two tensors overlaps.
@@ -430,144 +478,179 @@ bool overlaps(const torch::Tensor& a, const torch::Tensor& b) {
     return x.first < y.second && y.first < x.second;
 }
 
-// An output of rows `own`: contiguous, and sharing memory with no input but
-// `own` itself, element for element.
-void check_rows_output(const torch::Tensor& out, const torch::Tensor& own,
-                       std::initializer_list<const torch::Tensor*> others) {
-    TORCH_CHECK(out.device() == own.device() && out.is_contiguous() && out.scalar_type() == own.scalar_type() &&
-                    out.numel() == own.numel(),
-                "outputs must be contiguous, of their input's dtype and size, on its device");
-    TORCH_CHECK((out.data_ptr() == own.data_ptr() && own.is_contiguous()) || !overlaps(out, own),
-                "an output may only be its own contiguous input");
-    for (const auto* t : others) TORCH_CHECK(t == nullptr || !overlaps(out, *t), "an output overlaps another tensor of the call");
+// The output of rows `own`: a new tensor, or the given one, which shares memory with no
+// tensor of the call but `own` itself, element for element.
+torch::Tensor output_of(const OptTensor& given, const torch::Tensor& own, std::initializer_list<const torch::Tensor*> others) {
+    if (!given.has_value()) return at::empty(own.sizes(), own.options());
+    const auto& out = *given;
+    PD_VALUE(out.sizes() == own.sizes() && out.scalar_type() == own.scalar_type() && out.device() == own.device(),
+             "out must have its input's shape, dtype and device");
+    PD_VALUE(out.is_contiguous() && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
+             "out must be contiguous and 16-byte aligned");
+    PD_VALUE(!out.requires_grad(), "inference only: detach tensors requiring gradients");
+    PD_VALUE((out.data_ptr() == own.data_ptr() && own.is_contiguous()) || !overlaps(out, own),
+             "an output may share memory only with its own contiguous input");
+    for (const auto* t : others) PD_VALUE(t == nullptr || !overlaps(out, *t), "an output overlaps another tensor of the call");
+    return out;
 }
 
-const torch::Tensor* pointer(const c10::optional<torch::Tensor>& t) { return t.has_value() ? &*t : nullptr; }
+const int32_t* counts_of(const OptTensor& counts, int64_t batch, const torch::Tensor& like) {
+    if (!counts.has_value()) return nullptr;
+    PD_TYPE(counts->device() == like.device() && counts->scalar_type() == at::kInt && counts->is_contiguous(),
+            "counts must be a contiguous int32 tensor on the inputs' device");
+    PD_VALUE(counts->dim() == 1 && counts->size(0) == batch, "counts must be [B]");
+    return counts->data_ptr<int32_t>();
+}
 
-// Head norms and rotation of q and, if given, k.
-void rotate_heads(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions, bool per_token,
-                  c10::optional<torch::Tensor> frequencies, int64_t style, double scale,
-                  c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight, double eps,
-                  torch::Tensor q_out, c10::optional<torch::Tensor> k_out) {
-    const pd_token_rows q_rows = rows_of(q, q);
-    pd_token_rows k_rows{};
-    TORCH_CHECK(k.has_value() == k_out.has_value(), "k and its output come together");
-    check_rows_output(q_out, q, {pointer(k), pointer(k_out)});
+void check_scales(double k_scale, double v_scale) {
+    for (double s : {k_scale, v_scale})
+        PD_VALUE(s > 0 && static_cast<float>(s) > 0 && std::isfinite(static_cast<float>(s)), "k_scale and v_scale must be finite and positive");
+}
+
+// Head norms and rotation of q and, if given, k: their outputs, new or given.
+std::tuple<torch::Tensor, OptTensor> rotate_heads(torch::Tensor q, OptTensor k, torch::Tensor positions, OptTensor frequencies,
+                                                  int64_t style, double scale, OptTensor q_weight, OptTensor k_weight,
+                                                  double eps, OptTensor q_out, OptTensor k_out) {
+    const Rows q_rows = rows_of(q, q, "q");
+    Rows k_rows{};
     if (k.has_value()) {
-        k_rows = rows_of(*k, q);
-        check_rows_output(*k_out, *k, {&q, &q_out});
+        k_rows = rows_of(*k, q, "k");
+        PD_VALUE(k->dim() == q.dim() && k_rows.batch == q_rows.batch && k_rows.tokens == q_rows.tokens && k_rows.dim == q_rows.dim,
+                 "q and k must hold the same tokens and head_dim");
     }
-    TORCH_CHECK(positions.device() == q.device() && positions.is_contiguous() && positions.scalar_type() == at::kInt &&
-                    positions.numel() == (per_token ? q.size(0) * q.size(1) : q.size(0)),
-                "positions must be int32, one per sequence or token, on the inputs' device");
-    const pd_rotation r = rotation_of(frequencies, style, scale, q_weight, k_weight, eps, q);
-    TORCH_CHECK(!r.q_weight_per_head || q_weight->size(0) == q.size(2), "q_weight must be [D] or [H, D]");
-    TORCH_CHECK(!r.k_weight_per_head || (k.has_value() && k_weight->size(0) == k->size(2)), "k_weight must be [D] or [H, D]");
+    PD_TYPE(positions.device() == q.device() && positions.scalar_type() == at::kInt && positions.is_contiguous(),
+            "positions must be a contiguous int32 tensor on the inputs' device");
+    const bool per_token = positions.dim() == 2;
+    PD_VALUE((positions.dim() == 1 || (per_token && positions.size(1) == q_rows.tokens)) && positions.size(0) == q_rows.batch,
+             "positions must be [B] or [B, n]");
+    const pd_rotation r = rotation_of(frequencies, style, scale, q_weight, k_weight, eps, &q_rows,
+                                      k.has_value() ? &k_rows : nullptr, q, q_rows.dim);
+    PD_VALUE(k.has_value() || !k_out.has_value(), "out must give an output for each input");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
-    check_status(pd_rotate_heads(&r, &q_rows, k.has_value() ? &k_rows : nullptr, dtype_code(q),
-                                 positions.data_ptr<int32_t>(), per_token, q_out.data_ptr(),
-                                 k.has_value() ? k_out->data_ptr() : nullptr, static_cast<int>(q.size(0)),
-                                 static_cast<int>(q.size(1)), static_cast<int>(q.size(2)),
-                                 k.has_value() ? static_cast<int>(k->size(2)) : 0, static_cast<int>(q.size(3)),
-                                 current_stream(q)));
+    torch::Tensor q_result = output_of(q_out, q, {pointer(k), pointer(k_out), &positions});
+    OptTensor k_result;
+    if (k.has_value()) k_result = output_of(k_out, *k, {&q, &q_result, &positions});
+    check_status(pd_rotate_heads(&r, &q_rows.rows, k.has_value() ? &k_rows.rows : nullptr, dtype_code(q),
+                                 positions.data_ptr<int32_t>(), per_token, q_result.data_ptr(),
+                                 k.has_value() ? k_result->data_ptr() : nullptr, static_cast<int>(q_rows.batch),
+                                 static_cast<int>(q_rows.tokens), static_cast<int>(q_rows.heads),
+                                 static_cast<int>(k_rows.heads), static_cast<int>(q_rows.dim), current_stream(q)));
+    return {q_result, k_result};
 }
 
-// Paged append of normed and rotated keys and of values; max_context >= 0:
+// Paged append of normed and rotated keys and of values, and q beside them; max_context >= 0:
 // positions are lengths, advanced on the device (all or nothing per sequence).
-void append_rotated(c10::optional<torch::Tensor> q, torch::Tensor k_new, torch::Tensor v_new, torch::Tensor table,
-                    torch::Tensor positions, c10::optional<torch::Tensor> counts,
-                    c10::optional<torch::Tensor> frequencies, int64_t style, double scale,
-                    c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight, double eps,
-                    c10::optional<torch::Tensor> q_out, torch::Tensor k_cache, torch::Tensor v_cache, double k_scale,
-                    double v_scale, int64_t max_context) {
-    const pd_token_rows k_rows = rows_of(k_new, k_new), v_rows = rows_of(v_new, k_new);
-    pd_token_rows q_rows{};
-    const int64_t batch = k_new.size(0);
-    for (const auto& t : {k_cache, v_cache, table, positions}) {
-        TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.device() == k_new.device(),
-                    "all tensors must be contiguous GPU tensors on one device");
-    }
-    TORCH_CHECK(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes() && k_cache.size(2) == k_new.size(2) &&
-                    k_cache.size(3) == k_new.size(3) && v_new.sizes() == k_new.sizes() &&
-                    v_cache.scalar_type() == k_cache.scalar_type() && k_cache.size(0) <= INT32_MAX,
-                "expected k/v cache [P,T,KV,D] matching k_new/v_new [B,tokens,KV,D]");
-    TORCH_CHECK(table.dim() == 2 && table.size(0) == batch && positions.dim() == 1 && positions.size(0) == batch &&
-                    table.scalar_type() == at::kInt && positions.scalar_type() == at::kInt,
-                "table must be int32 [B, W] and positions int32 [B]");
-    if (counts.has_value()) {
-        TORCH_CHECK(counts->device() == k_new.device() && counts->is_contiguous() && counts->scalar_type() == at::kInt &&
-                        counts->dim() == 1 && counts->size(0) == batch,
-                    "counts must be int32 [B]");
-    }
-    TORCH_CHECK(!overlaps(k_cache, v_cache), "the caches overlap");
-    for (const auto* cache : {&k_cache, &v_cache})
-        for (const auto* t : {static_cast<const torch::Tensor*>(&k_new), static_cast<const torch::Tensor*>(&v_new), pointer(q), pointer(q_out)})
-            TORCH_CHECK(t == nullptr || !overlaps(*cache, *t), "the cache overlaps another tensor of the call");
-    TORCH_CHECK(q.has_value() == q_out.has_value(), "q and its output come together");
+OptTensor append_rotated(std::tuple<int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> layout, torch::Tensor k_cache,
+                         torch::Tensor v_cache, torch::Tensor table, torch::Tensor positions, torch::Tensor k_new,
+                         torch::Tensor v_new, OptTensor q, OptTensor frequencies, int64_t style, double scale,
+                         OptTensor q_weight, OptTensor k_weight, double eps, double k_scale, double v_scale, OptTensor counts,
+                         OptTensor out, int64_t max_context) {
+    const auto [batch, query_heads, kv_heads, dim, page_size, pages] = layout;
+    for (const auto* t : {&table, &positions})
+        PD_TYPE(t->device() == k_cache.device() && t->scalar_type() == at::kInt && t->is_contiguous(),
+                "table and positions must be contiguous int32 tensors on the cache device");
+    PD_VALUE(table.dim() == 2 && table.size(0) == batch && positions.dim() == 1 && positions.size(0) == batch &&
+                 table.size(1) >= 1 && table.size(1) <= 65536,
+             "table must be [B, W], at most 65536 wide, and positions [B]");
+    const Rows k_rows = rows_of(k_new, k_new, "k_new"), v_rows = rows_of(v_new, k_new, "v_new");
+    PD_VALUE(k_new.sizes() == v_new.sizes() && k_rows.batch == batch && k_rows.heads == kv_heads && k_rows.dim == dim,
+             "new tokens must be [B, Hkv, D] or [B, tokens, Hkv, D] matching the layout");
+    PD_VALUE(max_context < 0 || k_rows.tokens <= max_context, "more new tokens than the plan's reserved context");
+    Rows q_rows{};
     if (q.has_value()) {
-        q_rows = rows_of(*q, k_new);
-        check_rows_output(*q_out, *q, {&k_new, &v_new});
+        q_rows = rows_of(*q, k_new, "q");
+        PD_VALUE(q->dim() == k_new.dim() && q_rows.batch == batch && q_rows.tokens == k_rows.tokens &&
+                     q_rows.heads == query_heads && q_rows.dim == dim,
+                 "q must hold the new tokens' queries, [B, tokens, Hq, D] matching the layout");
+    } else {
+        PD_VALUE(!out.has_value() && !q_weight.has_value(), "q_weight and out need q");
     }
-    const pd_rotation r = rotation_of(frequencies, style, scale, q_weight, k_weight, eps, k_new);
-    TORCH_CHECK(!r.q_weight_per_head || (q.has_value() && q_weight->size(0) == q->size(2)), "q_weight must be [D] or [H, D]");
-    TORCH_CHECK(!r.k_weight_per_head || k_weight->size(0) == k_new.size(2), "k_weight must be [D] or [H, D]");
-    TORCH_CHECK(max_context <= (1 << 20), "max_context must not exceed 1048576");
+    for (const auto* c : {&k_cache, &v_cache}) {
+        PD_VALUE(c->dim() == 4 && c->size(0) == pages && c->size(1) == page_size && c->size(2) == kv_heads && c->size(3) == dim,
+                 "cache shape does not match the layout");
+        PD_TYPE(c->scalar_type() == k_cache.scalar_type() &&
+                    (c->scalar_type() == k_new.scalar_type() || (is_fp8(*c) && k_new.scalar_type() != at::kFloat)),
+                "the cache must have the new tokens' dtype, or float8_e4m3fn/float8_e5m2 under 16-bit tokens");
+        PD_VALUE(c->device() == k_new.device() && c->is_contiguous(), "cache tensors must be contiguous on the new tokens' device");
+        PD_VALUE(!c->requires_grad(), "inference only: detach tensors requiring gradients");
+    }
+    PD_VALUE(pages <= INT32_MAX && (page_size == 16 || page_size == 32), "page_size must be 16 or 32");
+    check_scales(k_scale, v_scale);
+    PD_VALUE(is_fp8(k_cache) || (k_scale == 1.0 && v_scale == 1.0), "k_scale and v_scale apply to FP8 caches");
+    const pd_rotation r = rotation_of(frequencies, style, scale, q_weight, k_weight, eps, q.has_value() ? &q_rows : nullptr,
+                                      &k_rows, k_new, dim);
+    const int32_t* count = counts_of(counts, batch, k_new);
+    PD_VALUE(!overlaps(k_cache, v_cache), "the caches overlap");
+    for (const auto* cache : {&k_cache, &v_cache})
+        for (const auto* t : {static_cast<const torch::Tensor*>(&k_new), static_cast<const torch::Tensor*>(&v_new), pointer(q),
+                              pointer(out)})
+            PD_VALUE(t == nullptr || !overlaps(*cache, *t), "the cache overlaps another tensor of the call");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(k_new.device());
-    const pd_token_rows* q_arg = q.has_value() ? &q_rows : nullptr;
-    void* q_dst = q.has_value() ? q_out->data_ptr() : nullptr;
-    const int32_t* count = counts.has_value() ? counts->data_ptr<int32_t>() : nullptr;
-    const int b = static_cast<int>(batch), n = static_cast<int>(k_new.size(1));
-    const int hq = q.has_value() ? static_cast<int>(q->size(2)) : 0, kv = static_cast<int>(k_new.size(2));
-    const int d = static_cast<int>(k_new.size(3)), page = static_cast<int>(k_cache.size(1));
-    const int width = static_cast<int>(table.size(1)), pages = static_cast<int>(k_cache.size(0));
+    OptTensor result;
+    if (q.has_value()) result = output_of(out, *q, {&k_new, &v_new, &table, &positions, pointer(counts)});
     const int dtype = dtype_code(k_new), cache_dtype = dtype_code(k_cache);
     const float ks = static_cast<float>(k_scale), vs = static_cast<float>(v_scale);
+    const pd_token_rows* q_arg = q.has_value() ? &q_rows.rows : nullptr;
+    void* q_dst = q.has_value() ? result->data_ptr() : nullptr;
+    const int b = static_cast<int>(batch), n = static_cast<int>(k_rows.tokens), hq = static_cast<int>(q_rows.heads);
+    const int kv = static_cast<int>(kv_heads), d = static_cast<int>(dim), page = static_cast<int>(page_size);
+    const int width = static_cast<int>(table.size(1)), all = static_cast<int>(pages);
     if (max_context >= 0) {
-        check_status(pd_append_rotated_advance(&r, q_arg, &k_rows, &v_rows, dtype, table.data_ptr<int32_t>(),
+        check_status(pd_append_rotated_advance(&r, q_arg, &k_rows.rows, &v_rows.rows, dtype, table.data_ptr<int32_t>(),
                                                positions.data_ptr<int32_t>(), count, q_dst, k_cache.data_ptr(),
-                                               v_cache.data_ptr(), cache_dtype, ks, vs, b, n, hq, kv, d, page, width,
-                                               pages, static_cast<int>(max_context), current_stream(k_new)));
+                                               v_cache.data_ptr(), cache_dtype, ks, vs, b, n, hq, kv, d, page, width, all,
+                                               static_cast<int>(max_context), current_stream(k_new)));
     } else {
-        check_status(pd_append_rotated(&r, q_arg, &k_rows, &v_rows, dtype, table.data_ptr<int32_t>(),
-                                       positions.data_ptr<int32_t>(), count, q_dst, k_cache.data_ptr(),
-                                       v_cache.data_ptr(), cache_dtype, ks, vs, b, n, hq, kv, d, page, width, pages,
-                                       current_stream(k_new)));
+        check_status(pd_append_rotated(&r, q_arg, &k_rows.rows, &v_rows.rows, dtype, table.data_ptr<int32_t>(),
+                                       positions.data_ptr<int32_t>(), count, q_dst, k_cache.data_ptr(), v_cache.data_ptr(),
+                                       cache_dtype, ks, vs, b, n, hq, kv, d, page, width, all, current_stream(k_new)));
     }
+    return result;
 }
 
-// Attention of several tokens per sequence (pd_decode_tokens).
-void decode_tokens(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lengths,
-                   c10::optional<torch::Tensor> counts, torch::Tensor out, torch::Tensor workspace, bool causal,
-                   double k_scale, double v_scale, c10::optional<torch::Tensor> length_bounds) {
-    for (const auto& t : {q, k, v, table, lengths, out, workspace}) {
-        TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.device() == q.device(),
-                    "all tensors must be contiguous GPU tensors on one device");
+// Attention of several tokens per sequence (pd_decode_tokens): out, or (none given) the
+// leading part of the plan's float32 buffer `own` as q's dtype.
+torch::Tensor decode_tokens(std::tuple<int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> layout, torch::Tensor q,
+                            torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lengths, OptTensor counts,
+                            OptTensor given, torch::Tensor own, torch::Tensor workspace, bool causal, double k_scale,
+                            double v_scale, OptTensor length_bounds) {
+    const auto [batch, query_heads, kv_heads, dim, page_size, pages] = layout;
+    PD_VALUE(q.dim() == 4 && q.size(0) == batch && q.size(1) >= 1 && q.size(1) <= own.size(1) && q.size(2) == query_heads && q.size(3) == dim,
+             "input shape does not match plan");
+    for (const auto* c : {&k, &v})
+        PD_VALUE(c->dim() == 4 && c->size(0) == pages && c->size(1) == page_size && c->size(2) == kv_heads && c->size(3) == dim,
+                 "input shape does not match plan");
+    PD_TYPE(token_type(q.scalar_type()) && v.scalar_type() == k.scalar_type() &&
+                (k.scalar_type() == q.scalar_type() || (is_fp8(k) && q.scalar_type() != at::kFloat)),
+            "q/k/v must share float16, bfloat16 or float32 dtype "
+            "(k/v may be float8_e4m3fn/float8_e5m2 with a float16 or bfloat16 q)");
+    check_scales(k_scale, v_scale);
+    for (const auto* t : {static_cast<const torch::Tensor*>(&q), static_cast<const torch::Tensor*>(&k),
+                          static_cast<const torch::Tensor*>(&v), pointer(given)}) {
+        if (t == nullptr) continue;
+        PD_VALUE(t->device() == table.device() && t->is_contiguous() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                 "inputs must be contiguous, 16-byte aligned, on the plan device");
+        PD_VALUE(!t->requires_grad(), "inference only: detach tensors requiring gradients");
     }
-    TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes() && k.size(3) == q.size(3) &&
-                    k.scalar_type() == v.scalar_type() && k.size(0) <= INT32_MAX,
-                "expected q[B,tokens,H,D], k/v[P,T,KV,D]");
-    TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out must be as q");
-    for (const auto* t : {&q, &k, &v}) TORCH_CHECK(!overlaps(out, *t), "out overlaps an input");
-    const int64_t batch = q.size(0);
-    TORCH_CHECK(table.dim() == 2 && table.size(0) == batch && lengths.dim() == 1 && lengths.size(0) == batch &&
-                    table.scalar_type() == at::kInt && lengths.scalar_type() == at::kInt,
-                "table must be int32 [B, W] and lengths int32 [B]");
-    if (counts.has_value()) {
-        TORCH_CHECK(counts->device() == q.device() && counts->is_contiguous() && counts->scalar_type() == at::kInt &&
-                        counts->dim() == 1 && counts->size(0) == batch,
-                    "counts must be int32 [B]");
+    const int32_t* count = counts_of(counts, batch, q);
+    torch::Tensor out;
+    if (given.has_value()) {
+        out = *given;
+        PD_VALUE(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out must have q's shape and dtype");
+    } else {
+        out = own.view(q.scalar_type()).view({-1}).narrow(0, 0, q.numel()).view(q.sizes());
     }
+    for (const auto* t : {&q, &k, &v}) PD_VALUE(!overlaps(out, *t), "out overlaps an input");
     const int32_t* bounds = bounds_pointer(length_bounds, batch);
     c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
     const size_t bytes = static_cast<size_t>(workspace.numel() * workspace.element_size());
     check_status(pd_decode_tokens(q.data_ptr(), dtype_code(q), k.data_ptr(), v.data_ptr(), dtype_code(k),
                                   static_cast<float>(k_scale), static_cast<float>(v_scale), table.data_ptr<int32_t>(),
-                                  lengths.data_ptr<int32_t>(), counts.has_value() ? counts->data_ptr<int32_t>() : nullptr,
-                                  out.data_ptr(), bytes > 0 ? workspace.data_ptr() : nullptr, bytes,
-                                  static_cast<int>(batch), static_cast<int>(q.size(1)), static_cast<int>(q.size(2)),
-                                  static_cast<int>(k.size(2)), static_cast<int>(q.size(3)), static_cast<int>(k.size(1)),
-                                  static_cast<int>(table.size(1)), static_cast<int>(k.size(0)), causal, bounds,
-                                  current_stream(q)));
+                                  lengths.data_ptr<int32_t>(), count, out.data_ptr(), bytes > 0 ? workspace.data_ptr() : nullptr,
+                                  bytes, static_cast<int>(batch), static_cast<int>(q.size(1)), static_cast<int>(query_heads),
+                                  static_cast<int>(kv_heads), static_cast<int>(dim), static_cast<int>(page_size),
+                                  static_cast<int>(table.size(1)), static_cast<int>(pages), causal, bounds, current_stream(q)));
+    return out;
 }
 
 // Workspace bytes of decode_tokens calls of up to `tokens` tokens, whatever their formats.

@@ -249,17 +249,11 @@ class DecodePlan:
         either way. No host synchronisation: it can be captured with ``run``
         and ``run_tokens``.
         """
-        from .rotary import launch_append
-
-        if k_new.device != self.device:
-            raise ValueError("cache and new tokens must be contiguous on the plan device")
-        tokens = k_new.shape[1] if k_new.dim() == 4 else 1
-        if tokens > self.context_capacity:
-            raise ValueError("more new tokens than the plan's reserved context")
-        out = launch_append(self.layout, k_cache, v_cache, self._table, self._lengths, k_new, v_new, rotary, q, q_weight,
-                            k_weight, eps, k_scale, v_scale, counts, out, self.context_capacity)
+        out = self._extension.append_rotated(dimensions(self.layout), k_cache, v_cache, self._table, self._lengths, k_new, v_new,
+                                             q, *rotation_arguments(rotary), q_weight, k_weight, eps, k_scale, v_scale, counts, out,
+                                             self.context_capacity)
         if self._bounds_known:
-            self._bounds.add_(tokens).clamp_(max=self.context_capacity)
+            self._bounds.add_(k_new.shape[1] if k_new.dim() == 4 else 1).clamp_(max=self.context_capacity)
         return out
 
     @property
@@ -274,7 +268,9 @@ class DecodePlan:
         if tuple(q.shape) != expected_q or tuple(k.shape) != expected_k or tuple(v.shape) != expected_k:
             raise ValueError("input shape does not match plan")
         _check_formats(q.dtype, k.dtype, v.dtype)
-        check_scales(k_scale, v_scale)
+        for scale in (k_scale, v_scale):
+            if isinstance(scale, bool) or not isinstance(scale, (int, float)) or not 0 < scale < math.inf:
+                raise ValueError("k_scale and v_scale must be finite and positive")
         for tensor in (q, k, v):
             if tensor.device != self.device or not tensor.is_contiguous():
                 raise ValueError("inputs must be contiguous on the plan device")
@@ -313,29 +309,9 @@ class DecodePlan:
         """
         if self.query_tokens is None:
             raise ValueError("the plan reserves no query tokens: build it with query_tokens")
-        layout = self.layout
-        expected_k = (layout.physical_pages, layout.page_size, layout.kv_heads, layout.head_dim)
-        if q.dim() != 4 or q.shape[0] != layout.batch or tuple(q.shape[2:]) != (layout.query_heads, layout.head_dim) or \
-                not 1 <= q.shape[1] <= self.query_tokens or tuple(k.shape) != expected_k or tuple(v.shape) != expected_k:
-            raise ValueError("input shape does not match plan")
-        _check_formats(q.dtype, k.dtype, v.dtype)
-        check_scales(k_scale, v_scale)
-        for tensor in (q, k, v) if out is None else (q, k, v, out):
-            if tensor.device != self.device or not tensor.is_contiguous():
-                raise ValueError("inputs must be contiguous on the plan device")
-            if tensor.requires_grad:
-                raise ValueError("inference only: detach tensors requiring gradients")
-        if counts is not None:
-            from .rotary import check_counts
-
-            check_counts(counts, layout.batch, self.device)
-        if out is None:
-            out = self._token_out.view(q.dtype).view(-1)[:q.numel()].view(q.shape)
-        elif out.shape != q.shape or out.dtype != q.dtype:
-            raise ValueError("out must have q's shape and dtype")
-        self._extension.decode_tokens(q, k, v, self._table, self._lengths, counts, out, self._token_workspace,
-                                      bool(causal), float(k_scale), float(v_scale), self._length_bounds())
-        return out
+        return self._extension.decode_tokens(dimensions(self.layout), q, k, v, self._table, self._lengths, counts, out,
+                                             self._token_out, self._token_workspace, causal, k_scale, v_scale,
+                                             self._length_bounds())
 
     def launches(self, q_dtype, kv_dtype=None):
         """Kernel launches ``run`` makes for q (and K/V) of these dtypes: 1 when the
@@ -483,10 +459,22 @@ def _check_formats(q_dtype, k_dtype, v_dtype):
                         "(k/v may be float8_e4m3fn/float8_e5m2 with a float16 or bfloat16 q)")
 
 
-def check_scales(k_scale, v_scale):
-    for scale in (k_scale, v_scale):
-        if isinstance(scale, bool) or not isinstance(scale, (int, float)) or not 0 < scale < math.inf:
-            raise ValueError("k_scale and v_scale must be finite and positive")
+_NO_ROTATION = (None, 0, 1.0)
+
+
+def rotation_arguments(rotary):
+    """A ``Rotary`` (or None) as the extension takes it: frequencies, style, scale."""
+    if rotary is None:
+        return _NO_ROTATION
+    arguments = getattr(rotary, "_arguments", None)
+    if arguments is None:
+        raise TypeError("rotary must be a Rotary or None")
+    return arguments
+
+
+def dimensions(layout):
+    """A layout's numbers, as the extension takes them."""
+    return (layout.batch, layout.query_heads, layout.kv_heads, layout.head_dim, layout.page_size, layout.physical_pages)
 
 
 def _check_cache(k_cache, v_cache, k_new, v_new, expected_k, device):

@@ -236,7 +236,7 @@ def test_refusals():
         rotate_heads(q, k, start, Rotary(frequencies(128)))               # more dims than the head
     with pytest.raises(ValueError):
         rotate_heads(q, k, start, rotary, q_weight=torch.ones(32, device="cuda", dtype=torch.float16))
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         rotate_heads(q, k, start, rotary, out=(q.view(-1)[:k.numel()].view(k.shape).new_empty(q.shape), q.view(-1)[:k.numel()].view(k.shape)))
     with pytest.raises(TypeError):
         append_rotated(layout, kc.float(), vc.float(), table, start, k, v, rotary)
@@ -244,7 +244,7 @@ def test_refusals():
         append_rotated(layout, kc, vc, table, start, k, v, rotary, k_scale=0.5)
     with pytest.raises(ValueError):
         append_rotated(layout, kc, vc, table, start, k, v[:, :3], rotary)
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         append_rotated(layout, kc, kc, table, start, k, v, rotary)
     with pytest.raises(TypeError):
         append_rotated(layout, kc, vc, table, start, k, v, rotary, counts=torch.ones(2, device="cuda"))

@@ -278,5 +278,5 @@ def test_refusals():
         plan.run_tokens(q, k, v, counts=torch.ones(3, dtype=torch.int32, device="cuda"))
     with pytest.raises(ValueError):
         plan.run_tokens(q, k, v, out=torch.empty_like(q, dtype=torch.float32))
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         plan.run_tokens(q, k, v, out=q)
