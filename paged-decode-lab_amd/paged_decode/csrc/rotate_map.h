@@ -40,16 +40,13 @@ struct RotateParams {
     int batch, tokens;
     int q_heads, kv_heads;   // as launched: 0 for q or k left out
     int heads;               // q_heads + kv_heads (+ kv_heads with a cache)
-    int head_groups;         // waves' head groups per token
-    int groups_per_wave;     // consecutive head groups of one token that a wave handles
-    int waves_per_token;
+    int head_groups;         // of a token: the heads that a wave holds at a time, a wave each
     int rotary_dim;          // 0: norm only
     int interleaved;
     int per_token_positions;
     int weight_f32;          // norm weights in FP32 (else the tokens' type)
     int q_weight_stride, k_weight_stride;  // elements between two heads' weights: 0 or D
-    int saturating;          // FP8 cache: largest finite value applies
-    float largest;
+    float largest;           // FP8 cache: its largest finite value
 };
 
 // Heads that one wave holds at a time.
