@@ -379,7 +379,7 @@ struct TokenRowsState {
     template <int NI>
     __device__ __forceinline__ void weigh(f32x4 (&s)[R][NI], int t0, bool masked, uint32_t invalid, float scale_log2, int lane) {
         const int quad = lane / 16;
-        float top[R];
+        float most[R];  // of the lane's own scores
         bool grow = false;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -392,18 +392,18 @@ struct TokenRowsState {
                         s[r][i][e] = seen ? s[r][i][e] : -INFINITY;
                     }
             }
-            float x = s[r][0][0];
+            most[r] = s[r][0][0];
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x = fmaxf(x, s[r][i][e]);
-            top[r] = max_over_lane_groups(x) * scale_log2;
-            grow |= top[r] > m[r] + Math::kSlack;
+                for (int e = 0; e < 4; ++e) most[r] = fmaxf(most[r], s[r][i][e]);
+            grow |= most[r] * scale_log2 > m[r] + Math::kSlack;
         }
-        if (__any(grow)) {
+        if (__any(grow)) {  // only then do a row's four lanes compare
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const float next = top[r] > m[r] + Math::kSlack ? top[r] - Math::kOffset : m[r];
+                const float top = max_over_lane_groups(most[r]) * scale_log2;
+                const float next = top > m[r] + Math::kSlack ? top - Math::kOffset : m[r];
                 const float alpha = fast_exp2(m[r] - next);
                 m[r] = next;
                 l[r] *= alpha;

@@ -15,6 +15,8 @@
 
 namespace pd {
 
+PD_HD int64_t lmax(int64_t a, int64_t b) { return a > b ? a : b; }
+
 struct TokenParams {
     const void* q;
     const void* k;
@@ -62,17 +64,21 @@ PD_HD int token_split(int splits, int split_tokens, int context) {
     return imax(split_tokens, (even + kTokenSplitUnit - 1) / kTokenSplitUnit * kTokenSplitUnit);
 }
 
-// Workgroup `block` of the launch (one grid dimension of batch * kv_heads *
-// splits * row_tiles): the tiles that see most come first.
+// Workgroup `block` of the launch (one grid dimension). Tiles that see most come
+// first, over all heads and splits, so that what remains at the end is short; a
+// (sequence, KV head, split) keeps its place modulo their number, so that with a multiple of
+// eight of them its tiles, which read the same K and V, run on one XCD.
 struct TokenCoords {
     int b, kv_head, split, tile;
 };
 
 PD_HD TokenCoords token_coords(const TokenParams& p, uint32_t block) {
-    const uint32_t unit = block / p.row_tiles;
+    const uint32_t units = static_cast<uint32_t>(p.batch * p.kv_heads * p.splits);
+    const uint32_t rank = block / units;
+    const uint32_t unit = block - rank * units;
     const uint32_t head = unit / p.splits;
     TokenCoords c;
-    c.tile = p.row_tiles - 1 - static_cast<int>(block - unit * p.row_tiles);
+    c.tile = p.row_tiles - 1 - static_cast<int>(rank);
     c.split = static_cast<int>(unit - head * p.splits);
     c.b = static_cast<int>(head / p.kv_heads);
     c.kv_head = static_cast<int>(head - static_cast<uint32_t>(c.b) * p.kv_heads);
@@ -80,7 +86,8 @@ PD_HD TokenCoords token_coords(const TokenParams& p, uint32_t block) {
 }
 
 // Stream kernel: workgroups of one split's KV heads are neighbours, wave w has
-// KV head w % head_waves of the workgroup's.
+// KV head w % head_waves of the workgroup's. Later splits, which short sequences
+// have nothing in, come last.
 PD_HD TokenCoords token_stream_coords(const TokenParams& p, uint32_t block, int wave) {
     const uint32_t head_groups = static_cast<uint32_t>(p.kv_heads / p.head_waves);
     const uint32_t unit = block / head_groups;
@@ -88,8 +95,8 @@ PD_HD TokenCoords token_stream_coords(const TokenParams& p, uint32_t block, int 
     TokenCoords c;
     c.kv_head = static_cast<int>(block - unit * head_groups) * p.head_waves + wave % p.head_waves;
     c.tile = static_cast<int>(unit - part * p.row_tiles);
-    c.b = static_cast<int>(part / p.splits);
-    c.split = static_cast<int>(part - static_cast<uint32_t>(c.b) * p.splits);
+    c.split = static_cast<int>(part / p.batch);
+    c.b = static_cast<int>(part - static_cast<uint32_t>(c.split) * p.batch);
     return c;
 }
 
@@ -133,14 +140,26 @@ struct TokenPlan {
     int64_t states;  // 0 with one split
 };
 
-constexpr int kTokenMinSplit = 256;    // cache tokens per split, at least
-constexpr int kTokenGroupsPerCu = 2;   // workgroups per CU that a split aims at
 constexpr int kStreamMaxRows = 32;     // rows that the stream kernel takes
 constexpr int kStreamWaves = 8;        // waves of its workgroups (FP32 rows are twice as long: 4)
+constexpr int kTokenMinSplit = 128;    // cache tokens per split, at least
+constexpr int kTokenGroupsPerCu = 2;   // workgroups per CU that splits of the tile kernel aim at
 
-// q_bytes: of a q element. bound: cache tokens the host knows no sequence to exceed.
+// The workgroups that a launch with splits of `span` tokens has anything to do in.
+inline int64_t live_splits(const int32_t* bounds, int batch, int64_t bound, int64_t span) {
+    if (bounds == nullptr) return batch * ((bound + span - 1) / span);
+    int64_t live = 0;
+    for (int b = 0; b < batch; ++b) live += (lmin(imax(bounds[b], 0), bound) + span - 1) / span;
+    return live;
+}
+
+// Splits that `unsplit` workgroups are cut into at most: 1 if they fill the device.
+inline int64_t token_most_splits(int64_t unsplit, int64_t wanted) { return unsplit >= wanted ? 1 : 4 * wanted / unsplit; }
+
+// q_bytes: of a q element. bound: cache tokens the host knows no sequence to
+// exceed; bounds: and each of them (or null).
 inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads, int64_t bound,
-                             int64_t max_states, int compute_units) {
+                             const int32_t* bounds, int64_t max_states, int compute_units) {
     TokenPlan t{};
     const int64_t rows = static_cast<int64_t>(tokens) * (query_heads / kv_heads);
     t.stream = rows <= kStreamMaxRows;
@@ -154,37 +173,48 @@ inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, i
         t.head_waves = 1;
     }
     t.row_tiles = static_cast<int>((rows + t.tile_rows - 1) / t.tile_rows);
-    const int64_t units = static_cast<int64_t>(batch) * kv_heads * t.row_tiles;
-    const int64_t groups = units / t.head_waves;
+    // Workgroups of one sequence's split, and how many the device should get.
+    const int64_t each = static_cast<int64_t>(kv_heads / t.head_waves) * t.row_tiles;
     const int64_t wanted = static_cast<int64_t>(compute_units) * (t.stream ? 1 : kTokenGroupsPerCu);
-    int64_t splits = groups < wanted ? (wanted + groups - 1) / groups : 1;
-    splits = lmin(splits, lmin((bound + kTokenMinSplit - 1) / kTokenMinSplit, max_states / (units * t.tile_rows)));
-    t.splits = 1;
-    t.split_tokens = kTokenSplitUnit;
-    if (splits > 1) {
-        const int64_t even = (bound + splits - 1) / splits;
-        t.split_tokens = static_cast<int>((even + kTokenSplitUnit - 1) / kTokenSplitUnit * kTokenSplitUnit);
-        t.splits = static_cast<int>((bound + t.split_tokens - 1) / t.split_tokens);
+    const int64_t states = static_cast<int64_t>(batch) * kv_heads * t.row_tiles * t.tile_rows;  // of one split
+    // The shortest split with which the workgroups still fit the device at once; those that find nothing to do,
+    // a short sequence's in later splits, count a quarter.
+    const int64_t limit = lmin(token_most_splits(each * batch, wanted), max_states / states);
+    int64_t span = bound;
+    if (limit > 1) {
+        const int64_t least = lmax(kTokenMinSplit, (bound + limit - 1) / limit);
+        int64_t low = (least + kTokenSplitUnit - 1) / kTokenSplitUnit, high = (bound + kTokenSplitUnit - 1) / kTokenSplitUnit;
+        while (low < high) {  // units of tokens; more of them, fewer workgroups
+            const int64_t mid = (low + high) / 2;
+            if (each * live_splits(bounds, batch, bound, mid * kTokenSplitUnit) <= wanted) high = mid;
+            else low = mid + 1;
+        }
+        span = low * kTokenSplitUnit;
     }
-    t.workgroups = groups * t.splits;
-    t.states = t.splits > 1 ? units * t.tile_rows * t.splits : 0;
+    t.splits = static_cast<int>((bound + span - 1) / span);
+    t.split_tokens = t.splits > 1 ? static_cast<int>(span) : kTokenSplitUnit;
+    t.workgroups = each * batch * t.splits;
+    t.states = t.splits > 1 ? states * t.splits : 0;
     return t;
 }
 
-// States with which no call of up to `tokens` tokens splits less than it would with more.
+// States with which no call of up to `tokens` tokens splits less than it would with
+// more: a split has at least kTokenMinSplit tokens, and unsplit calls at least `wanted` workgroups.
 inline int64_t most_token_states(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads, int64_t reach,
                                  int compute_units) {
-    int64_t states = 0;
+    int64_t most = 0;
     for (int n = 1; n <= tokens; ++n) {
-        const TokenPlan t = plan_tokens(q_bytes, head_dim, batch, n, query_heads, kv_heads, reach, INT64_MAX, compute_units);
-        const int64_t units = t.workgroups / t.splits * t.head_waves;
-        const int64_t wanted = static_cast<int64_t>(compute_units) * (t.stream ? 1 : kTokenGroupsPerCu) * t.head_waves;
-        if (units >= wanted && !t.stream) break;  // and so for every larger n
-        // A shorter context takes at most these splits, rounded to whole units of tokens.
-        const int64_t most = lmin((wanted + units - 1) / units, (reach + kTokenMinSplit - 1) / kTokenMinSplit);
-        if (most > 1 && most * units * t.tile_rows > states) states = most * units * t.tile_rows;
+        const TokenPlan t = plan_tokens(q_bytes, head_dim, batch, n, query_heads, kv_heads, reach, nullptr, 0, compute_units);
+        const int64_t wanted = static_cast<int64_t>(compute_units) * (t.stream ? 1 : kTokenGroupsPerCu);
+        if (t.workgroups >= wanted) {
+            if (t.stream) continue;
+            break;  // and so for every larger n
+        }
+        const int64_t splits = lmin(token_most_splits(t.workgroups, wanted), (reach + kTokenMinSplit - 1) / kTokenMinSplit);
+        const int64_t states = static_cast<int64_t>(batch) * kv_heads * t.row_tiles * t.tile_rows;
+        if (splits > 1 && splits * states > most) most = splits * states;
     }
-    return states;
+    return most;
 }
 
 }  // namespace pd
