@@ -48,7 +48,7 @@ struct TokenMath<_Float16> {
         }
         return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
     }
-    static constexpr uint32_t kExponents = 0x7C007C00u, kExponent = 0x7C00u;
+    static constexpr uint32_t kExponents = 0x7C007C00u, kLast = 0x04000400u;  // and their last bits
 };
 
 template <>
@@ -62,20 +62,18 @@ struct TokenMath<__bf16> {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
     }
     template <int KVF>
-    static __device__ __forceinline__ u32x2 widen(uint32_t w) {  // FP8 values are the top halves of their FP32 form
-        f32x2 a, b;
+    static __device__ __forceinline__ u32x2 widen(uint32_t w) {
+        bf16x2 a, b;
         if constexpr (KVF == PD_DTYPE_FP8_E4M3) {
-            a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
-            b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+            a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+            b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
         } else {
-            a = __builtin_amdgcn_cvt_pk_f32_bf8(w, false);
-            b = __builtin_amdgcn_cvt_pk_f32_bf8(w, true);
+            a = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, false);
+            b = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, true);
         }
-        const float a0 = a[0], a1 = a[1], b0 = b[0], b1 = b[1];
-        return u32x2{(__builtin_bit_cast(uint32_t, a0) >> 16) | (__builtin_bit_cast(uint32_t, a1) & 0xFFFF0000u),
-                     (__builtin_bit_cast(uint32_t, b0) >> 16) | (__builtin_bit_cast(uint32_t, b1) & 0xFFFF0000u)};
+        return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
     }
-    static constexpr uint32_t kExponents = 0x7F807F80u, kExponent = 0x7F80u;
+    static constexpr uint32_t kExponents = 0x7F807F80u, kLast = 0x00800080u;  // and their last bits
 };
 
 template <>
@@ -83,18 +81,17 @@ struct TokenMath<float> {
     static constexpr float kOffset = 0.0f, kSlack = 8.0f;
 };
 
-// Whether a 16-byte chunk holds an infinity or a NaN.
-template <typename QT>
+// Whether a 16-byte chunk of QT values, or of FP8 ones as stored (KVF), holds an
+// infinity or a NaN: an exponent (E4M3: all bits but the sign) of ones, which one more carries into the sign's place.
+template <typename QT, int KVF>
 __device__ __forceinline__ bool holds_nonfinite(const u32x4& w) {
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(QT) == 4) {
-            bad |= (w[i] & 0x7F800000u) == 0x7F800000u;
-        } else {
-            constexpr uint32_t kLow = TokenMath<QT>::kExponent, kHigh = kLow << 16;
-            bad |= (w[i] & kLow) == kLow || (w[i] & kHigh) == kHigh;
-        }
+        if constexpr (KVF == PD_DTYPE_FP8_E4M3) bad |= (((w[i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
+        else if constexpr (KVF == PD_DTYPE_FP8_E5M2) bad |= (((w[i] & 0x7C7C7C7Cu) + 0x04040404u) & 0x80808080u) != 0;
+        else if constexpr (sizeof(QT) == 4) bad |= (w[i] & 0x7F800000u) == 0x7F800000u;
+        else bad |= (((w[i] & TokenMath<QT>::kExponents) + TokenMath<QT>::kLast) & 0x80008000u) != 0;
     }
     return bad;
 }
@@ -118,9 +115,17 @@ __device__ __forceinline__ u32x2 transposed_read(const char* p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec*)p));
 }
 
+// The same of bytes: each 16 lanes address eight rows of 16 bytes (lane i: row
+// i / 2, bytes 8 (i % 2) on), and lane i gets byte i of each row.
+__device__ __forceinline__ u32x2 transposed_bytes(const char* p) {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i32x2 LdsVec;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsVec*)p));
+}
+
 // What a workgroup of the kernel works on.
 struct TokenWork {
-    int b, kv_head, split;
+    int b, kv_head, item;
     int row0;       // first row of the tile
     int rows;       // live rows of the sequence (tokens x group)
     int count, context;
@@ -149,7 +154,7 @@ __device__ __forceinline__ void token_rows_one_by_one(const TokenParams& p, cons
     for (int i = first; i < rows; i += step) {
         const int row = w.row0 + i;
         if (row >= w.rows) {
-            if (p.splits == 1) store_row_zeros<QT, D>(p, w, row, lane);
+            if (p.split == kTokenWhole) store_row_zeros<QT, D>(p, w, row, lane);
             continue;
         }
         const int token = row / p.group;
@@ -176,13 +181,13 @@ __device__ __forceinline__ void token_rows_one_by_one(const TokenParams& p, cons
 #pragma unroll
             for (int e = 0; e < PER; ++e) o[e] = o[e] * alpha + weight * stored_value<QT, KVF>(v_head + offset, lane * PER + e);
         }
-        if (p.splits == 1) {
+        if (p.split == kTokenWhole) {
             const float inv = l == 0.0f ? 0.0f : p.v_scale / l;
 #pragma unroll
             for (int e = 0; e < PER; ++e)
                 static_cast<QT*>(p.out)[at + lane * PER + e] = static_cast<QT>(l == 0.0f ? 0.0f : o[e] * inv);
         } else {
-            const int64_t state = token_state(p, w.b, w.kv_head, row, w.split);
+            const int64_t state = token_state(p, w.item, w.kv_head, row);
 #pragma unroll
             for (int e = 0; e < PER; ++e) p.numerator[state * D + lane * PER + e] = o[e] * p.v_scale;
             if (lane == 0) *reinterpret_cast<float2*>(p.stats + state * 2) = make_float2(m, l);
@@ -244,19 +249,19 @@ __device__ __forceinline__ RowBlock row_block(const TokenParams& p, int page, in
     return {row * p.kv_row_bytes, valid ? static_cast<uint32_t>(imin(end - t, 16)) * p.kv_row_bytes : 0u};
 }
 
-// A tile of KT cache tokens of K or V on its way into LDS, by WAVES waves. 16- and
-// 32-bit caches go there directly; FP8 ones through registers (raw), where they
-// are widened when they `land`.
-template <typename QT, int KVF, int D, int WAVES, int KT>
+// A tile of KT cache tokens of K or V on its way into LDS, by WAVES waves. It
+// goes there directly, as stored, or (kWiden, FP8) through registers, where it is
+// widened when it lands.
+template <typename QT, int KVF, int D, int WAVES, int KT, bool kWiden>
 struct TileLoad {
-    static constexpr bool kWiden = KVF != kTokenNative;
-    static constexpr int ES = kWiden ? 1 : static_cast<int>(sizeof(QT));
-    static constexpr int RB = D * static_cast<int>(sizeof(QT));  // bytes of a row in LDS
-    static constexpr int SB = D * ES;                            // and in the cache
+    static constexpr bool kFp8 = KVF != kTokenNative;
+    static constexpr int SB = D * (kFp8 ? 1 : static_cast<int>(sizeof(QT)));            // bytes of a row in the cache
+    static constexpr int RB = kWiden ? D * static_cast<int>(sizeof(QT)) : SB;           // and in LDS
     static constexpr int RPI = 1024 / SB;                        // rows per request of a wave
     static constexpr int NL = KT * SB / 1024 / WAVES;            // requests per wave
     static constexpr int LPR = SB / 16;                          // lanes per row
     static_assert(NL * WAVES * 1024 == KT * SB && 16 % RPI == 0, "whole requests, within 16 tokens");
+    static_assert(!kWiden || kFp8, "what is widened");
     u32x4 raw[kWiden ? NL : 1];
 
     // ids: tile_pages of the tile; head: the cache from its KV head on; to: the tile's address in LDS.
@@ -283,7 +288,7 @@ struct TileLoad {
             raw[kPart] = __builtin_amdgcn_raw_buffer_load_b128(row_buffer(head + rows.offset, rows.bytes), offset, 0, 0);
         } else {
             // LDS slot `lane` of the request holds the chunk that token_chunk puts there.
-            const uint32_t offset = r * p.kv_row_bytes + token_slot_chunk<RB>(r, lane % LPR) * 16;
+            const uint32_t offset = r * p.kv_row_bytes + token_slot_chunk<RB, kFp8>(row0 + lane / LPR, lane % LPR) * 16;
             load_to_lds<kPart * WAVES * RPI * RB>(head + rows.offset, rows.bytes, to, offset);
         }
     }
@@ -313,12 +318,13 @@ __device__ __forceinline__ uint32_t invalid_blocks(const TokenParams& p, int ids
 }
 
 // A wave's R blocks of 16 rows: q as the first product's operand, what the rows
-// see, and their softmax state.
-template <typename QT, int D, int R>
+// see, and their softmax state. KVF: FP8 format of the tiles in LDS, if they are that.
+template <typename QT, int KVF, int D, int R>
 struct TokenRowsState {
     static constexpr bool kF32 = sizeof(QT) == 4;
-    static constexpr int RB = D * static_cast<int>(sizeof(QT));
-    static constexpr int KS = RB / 64;  // steps of four chunks of the first product
+    static constexpr bool kFp8 = KVF != kTokenNative;
+    static constexpr int RB = D * (kFp8 ? 1 : static_cast<int>(sizeof(QT)));
+    static constexpr int KS = D * static_cast<int>(sizeof(QT)) / 64;  // steps of four chunks of the first product
     static constexpr int ND = D / 16;   // blocks of 16 dims of the second
     using Math = TokenMath<QT>;
     u32x4 q[R][KS];
@@ -359,7 +365,15 @@ struct TokenRowsState {
             for (int r = 0; r < R; ++r) s[r][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(k_tile + token_chunk<RB>(16 * i + col, 4 * ks + quad) * 16);
+                u32x4 kf;
+                if constexpr (kFp8) {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(
+                        k_tile + token_chunk<RB, true>(16 * i + col, 2 * ks + quad / 2) * 16 + (quad % 2) * 8);
+                    const u32x2 a = Math::template widen<KVF>(w[0]), b = Math::template widen<KVF>(w[1]);
+                    kf = u32x4{a[0], a[1], b[0], b[1]};
+                } else {
+                    kf = *reinterpret_cast<const u32x4*>(k_tile + token_chunk<RB>(16 * i + col, 4 * ks + quad) * 16);
+                }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if constexpr (kF32) {
@@ -450,13 +464,21 @@ struct TokenRowsState {
                 }
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    // Lane (col, quad) gets dim 16 d + col of tokens 4 quad .. + 3, by a transposing read: the 16 lanes of a
-                    // quad address four rows of four 8-byte pieces.
-                    const int row = 32 * u + 4 * quad + col / 4;
-                    const int piece = 2 * d + (col % 4) / 2;
-                    const u32x2 v0 = transposed_read(v_tile + token_chunk<RB>(row, piece) * 16 + (col % 2) * 8);
-                    const u32x2 v1 = transposed_read(v_tile + token_chunk<RB>(row + 16, piece) * 16 + (col % 2) * 8);
-                    const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
+                    // Lane (col, quad) gets dim 16 d + col of tokens 4 quad .. + 3 and of those 16 behind, by transposing
+                    // reads: the 16 lanes of a quad address four rows of four 8-byte pieces (FP8: all eight rows).
+                    u32x4 vf;
+                    if constexpr (kFp8) {
+                        const int row = 32 * u + 4 * quad + (col / 2) % 4 + (col / 8) * 16;
+                        const u32x2 w = transposed_bytes(v_tile + token_chunk<RB, true>(row, d) * 16 + (col % 2) * 8);
+                        const u32x2 a = Math::template widen<KVF>(w[0]), b = Math::template widen<KVF>(w[1]);
+                        vf = u32x4{a[0], a[1], b[0], b[1]};
+                    } else {
+                        const int row = 32 * u + 4 * quad + col / 4;
+                        const int piece = 2 * d + (col % 4) / 2;
+                        const u32x2 v0 = transposed_read(v_tile + token_chunk<RB>(row, piece) * 16 + (col % 2) * 8);
+                        const u32x2 v1 = transposed_read(v_tile + token_chunk<RB>(row + 16, piece) * 16 + (col % 2) * 8);
+                        vf = u32x4{v0[0], v0[1], v1[0], v1[1]};
+                    }
 #pragma unroll
                     for (int r = 0; r < R; ++r) o[r][d] = Math::mma(vf, wt[r], o[r][d]);
                 }
@@ -474,22 +496,64 @@ __device__ __forceinline__ TokenParams reloaded_params() {
     return *(const TokenParams*)p;
 }
 
+// Where an item's splits lie: its sequence and the tokens of a split.
+struct TokenItem {
+    int b, first;  // the sequence, and its first item
+    int span;
+};
+
+// Sums of x over lanes 0 .. lane.
+__device__ __forceinline__ int wave_prefix(int x, int lane) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const int y = __shfl_up(x, d);
+        x += lane >= d ? y : 0;
+    }
+    return x;
+}
+
+// The list of splits, a sequence a lane: splits that end at or before this lane's
+// sequence, and the span with which all of them fit p.items.
+__device__ __forceinline__ int token_list(const TokenParams& p, int lane, int& span) {
+    const int context = lane < p.batch ? token_context(p, lane) : 0;
+    for (span = p.split_tokens;; span *= 2) {  // ends: with one split each there are no more than sequences
+        const int upto = wave_prefix(token_ceil(context, span), lane);
+        if (__builtin_amdgcn_readlane(upto, kWave - 1) <= p.items) return upto;
+    }
+}
+
+// The sequence of `item` (b = batch if the list is shorter).
+__device__ __forceinline__ TokenItem token_item(const TokenParams& p, int item, int lane) {
+    TokenItem t;
+    if (p.split == kTokenList) {
+        const int upto = token_list(p, lane, t.span);
+        t.b = imin(__popcll(__ballot(lane < p.batch && upto <= item)), p.batch);
+        t.first = t.b > 0 ? __builtin_amdgcn_readlane(upto, t.b - 1) : 0;
+    } else {
+        const int splits = p.items / p.batch;
+        t.b = item / splits;
+        t.first = t.b * splits;
+        t.span = p.split == kTokenWhole ? p.split_tokens : token_grid_span(splits, p.split_tokens, token_context(p, t.b));
+    }
+    return t;
+}
+
 // The work of a workgroup whose tile has M rows from row0 on; false if no row of it
 // sees a token of its split.
 template <int M>
-__device__ __forceinline__ bool open_work(const TokenParams& p, const TokenCoords& at, TokenWork& w, int& last) {
-    w.b = at.b;
+__device__ __forceinline__ bool open_work(const TokenParams& p, const TokenCoords& at, TokenWork& w, int& last, int lane) {
+    const TokenItem t = token_item(p, at.item, lane);
+    w.b = imin(t.b, p.batch - 1);
+    w.item = at.item;
     w.kv_head = at.kv_head;
-    w.split = at.split;
     w.row0 = at.tile * M;
     w.count = token_count(p, w.b);
     w.context = token_context(p, w.b);
     w.rows = w.count * p.group;
     last = imin(w.row0 + M, w.rows) - 1;
-    const int span = token_split(p.splits, p.split_tokens, w.context);
-    w.begin = w.split * span;
-    w.end = last < w.row0 ? 0 : imin(w.begin + span, token_sees(p.causal, w.context, w.count, last / p.group));
-    return w.begin < w.end;
+    w.begin = (at.item - t.first) * t.span;
+    w.end = last < w.row0 ? 0 : imin(w.begin + t.span, token_sees(p.causal, w.context, w.count, last / p.group));
+    return t.b < p.batch && w.begin < w.end;
 }
 
 // ---------------------------------------------------------------------------
@@ -498,8 +562,8 @@ __device__ __forceinline__ bool open_work(const TokenParams& p, const TokenCoord
 // next is on its way while one is used.
 template <typename QT, int KVF, int D, int R, int WAVES, int KT>
 __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenParams p) {
-    using Rows = TokenRowsState<QT, D, R>;
-    using Load = TileLoad<QT, KVF, D, WAVES, KT>;
+    using Rows = TokenRowsState<QT, kTokenNative, D, R>;
+    using Load = TileLoad<QT, KVF, D, WAVES, KT, KVF != kTokenNative>;
     constexpr int RB = Rows::RB;
     constexpr int M = WAVES * R * 16;
     constexpr int TILE = KT * RB;
@@ -510,8 +574,8 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     TokenWork w;
     int last;
-    if (!open_work<M>(p, token_coords(p, blockIdx.x), w, last)) {
-        if (p.splits == 1)  // states of such splits are never read
+    if (!open_work<M>(p, token_coords(p, blockIdx.x), w, last, lane)) {
+        if (p.split == kTokenWhole)  // states of such splits are never read
             for (int i = wave; i < M; i += WAVES) store_row_zeros<QT, D>(p, w, w.row0 + i, lane);
         return;
     }
@@ -548,7 +612,7 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
         if (t0 + KT > common) {  // uniform
             bool bad = false;
             for (int i = threadIdx.x; i < TILE / 16; i += WAVES * kWave)
-                bad |= holds_nonfinite<QT>(*reinterpret_cast<const u32x4*>(v_tile + i * 16));
+                bad |= holds_nonfinite<QT, kTokenNative>(*reinterpret_cast<const u32x4*>(v_tile + i * 16));
             if (__syncthreads_or(bad)) {
                 wait_for_loads();
                 token_rows_one_by_one<QT, KVF, D>(p, w, M, wave, WAVES, lane);
@@ -568,7 +632,7 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
         const float sum = sum_over_lane_groups(rows.l[r]);
         const int row = w.row0 + (wave * R + r) * 16 + col;
         const int token = row / p.group;
-        if (p.splits == 1) {
+        if (p.split == kTokenWhole) {
             if (token >= p.tokens) continue;
             const float inv = sum == 0.0f ? 0.0f : p.v_scale / sum;
             QT* out = static_cast<QT*>(p.out) + token_q_row(p, w.b, w.kv_head, token, row - token * p.group) * D;
@@ -583,7 +647,7 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
                         u32x2{Rows::Math::pack(x[0], x[1]), Rows::Math::pack(x[2], x[3])};
             }
         } else if (row < w.rows) {
-            const int64_t state = token_state(p, w.b, w.kv_head, row, w.split);
+            const int64_t state = token_state(p, w.item, w.kv_head, row);
 #pragma unroll
             for (int d = 0; d < Rows::ND; ++d)
                 *reinterpret_cast<f32x4*>(p.numerator + state * D + 16 * d + 4 * quad) = rows.o[r][d] * p.v_scale;
@@ -593,15 +657,15 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: every wave streams cache tokens of its own, tiles of 32 from
+// Few rows: every wave streams cache tokens of its own, tiles of 32 or 64 from
 // its part of LDS, for all R blocks of 16 rows, and the workgroup's waves of
 // one KV head combine at the end. The next K is requested once a tile is scored,
 // the next V once it is added, so that a wave always has loads in flight.
 template <typename QT, int KVF, int D, int R, int WAVES>
 struct StreamShape {
-    static constexpr int KT = 32;
-    static constexpr int RB = D * static_cast<int>(sizeof(QT));
-    static constexpr int TILE = KT * RB;
+    static constexpr int SB = D * (KVF == kTokenNative ? static_cast<int>(sizeof(QT)) : 1);
+    static constexpr int KT = SB >= 256 ? 32 : 64;  // so that a wave's tile of K and V is 8 to 32 KB
+    static constexpr int TILE = KT * SB;
     static constexpr int SD = D + 4;  // floats from one row's sums to the next: rows begin in other banks
     static constexpr int STATE = R * 16 * SD * 4;
     static constexpr int REGION = 2 * TILE > STATE ? 2 * TILE : STATE;
@@ -609,10 +673,10 @@ struct StreamShape {
 
 template <typename QT, int KVF, int D, int R, int WAVES>
 __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const TokenParams p) {
-    using Rows = TokenRowsState<QT, D, R>;
+    using Rows = TokenRowsState<QT, KVF, D, R>;
     using Shape = StreamShape<QT, KVF, D, R, WAVES>;
     constexpr int KT = Shape::KT;
-    using Load = TileLoad<QT, KVF, D, 1, KT>;
+    using Load = TileLoad<QT, KVF, D, 1, KT, false>;
     constexpr int M = R * 16;
     __shared__ __attribute__((aligned(1024))) char regions[WAVES * Shape::REGION];
     __shared__ float2 states[WAVES][M];
@@ -623,8 +687,8 @@ __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const Token
     const int slice = wave / p.head_waves, slices = WAVES / p.head_waves;
     TokenWork w;
     int last;
-    if (!open_work<M>(p, at, w, last)) {  // the same for all waves
-        if (p.splits == 1)
+    if (!open_work<M>(p, at, w, last, lane)) {  // the same for all waves
+        if (p.split == kTokenWhole)
             for (int i = slice; i < M; i += slices) store_row_zeros<QT, D>(p, w, w.row0 + i, lane);
         return;
     }
@@ -652,29 +716,21 @@ __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const Token
         const bool masked = t0 + KT > common || invalid != 0 || partial;
         f32x4 s[R][KT / 16];
         // Requests behind the end have no rows: they write zeros that nothing reads, and keep the counts the same.
-        if constexpr (!Load::kWiden) wait_for_loads<Load::NL>();  // all but V's
-        k_load.land(k_tile, 0, lane);
+        wait_for_loads<Load::NL>();  // all but V's
         const int later_ids = tile_pages<KT>(p, pages, t0 + 2 * step, lane);
-        if constexpr (Load::kWiden) k_load.request(p, next_ids, k_head, k_at, t0 + step, w.end, 0, lane);
         rows.score(k_tile, s, lane);
-        if constexpr (!Load::kWiden) {
-            wait_for_reads();
-            k_load.request(p, next_ids, k_head, k_at, t0 + step, w.end, 0, lane);
-        }
+        wait_for_reads();
+        k_load.request(p, next_ids, k_head, k_at, t0 + step, w.end, 0, lane);
         rows.weigh(s, t0, masked, invalid, p.scale_log2, lane);
-        if constexpr (!Load::kWiden) wait_for_loads<Load::NL>();  // all but the next K's
-        v_load.land(v_tile, 0, lane);
-        if constexpr (Load::kWiden) v_load.request(p, next_ids, v_head, v_at, t0 + step, w.end, 0, lane);
+        wait_for_loads<Load::NL>();  // all but the next K's
         if (t0 + KT > common) {
             for (int i = lane; i < Shape::TILE / 16; i += kWave)
-                bad |= holds_nonfinite<QT>(*reinterpret_cast<const u32x4*>(v_tile + i * 16));
+                bad |= holds_nonfinite<QT, KVF>(*reinterpret_cast<const u32x4*>(v_tile + i * 16));
             if (__any(bad)) break;
         }
         rows.add(v_tile, s, lane);
-        if constexpr (!Load::kWiden) {
-            wait_for_reads();
-            v_load.request(p, next_ids, v_head, v_at, t0 + step, w.end, 0, lane);
-        }
+        wait_for_reads();
+        v_load.request(p, next_ids, v_head, v_at, t0 + step, w.end, 0, lane);
         ids = next_ids;
         next_ids = later_ids;
     }
@@ -714,13 +770,13 @@ __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const Token
 #pragma unroll
             for (int e = 0; e < PER; ++e) o[e] = fmaf(from[e], a, o[e]);
         }
-        if (late.splits == 1) {
+        if (late.split == kTokenWhole) {
             QT* out = static_cast<QT*>(late.out) + token_q_row(late, w.b, w.kv_head, token, row - token * late.group) * D + lane * PER;
             const float inv = l == 0.0f ? 0.0f : late.v_scale / l;
 #pragma unroll
             for (int e = 0; e < PER; ++e) out[e] = static_cast<QT>(l == 0.0f ? 0.0f : o[e] * inv);
         } else if (row < w.rows) {
-            const int64_t state = token_state(late, w.b, w.kv_head, row, w.split);
+            const int64_t state = token_state(late, w.item, w.kv_head, row);
 #pragma unroll
             for (int e = 0; e < PER; ++e) late.numerator[state * D + lane * PER + e] = o[e] * late.v_scale;
             if (lane == 0) *reinterpret_cast<float2*>(late.stats + state * 2) = make_float2(m, l);
@@ -738,31 +794,40 @@ __global__ void __launch_bounds__(256) token_merge_kernel(const TokenParams p) {
     constexpr int SPW = kWave / LPS;    // states per read
     constexpr int kUnroll = 4;
     const int lane = threadIdx.x % kWave;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens * p.query_heads;
     if (item >= rows) return;
     const uint32_t bt = static_cast<uint32_t>(item / p.query_heads);
     const int head = static_cast<int>(item - static_cast<int64_t>(bt) * p.query_heads);
     const int b = static_cast<int>(bt / p.tokens), token = static_cast<int>(bt - static_cast<uint32_t>(b) * p.tokens);
     const int kv_head = head / p.group;
+    int first, span;  // the sequence's splits
+    if (p.split == kTokenList) {
+        const int upto = token_list(p, lane, span);
+        first = b > 0 ? __builtin_amdgcn_readlane(upto, b - 1) : 0;
+    } else {
+        const int splits = p.items / p.batch;
+        first = b * splits;
+        span = token_grid_span(splits, p.split_tokens, token_context(p, b));
+    }
     const int count = token_count(p, b), context = token_context(p, b);
     const int sees = token < count ? token_sees(p.causal, context, count, token) : 0;
-    const int span = token_split(p.splits, p.split_tokens, context);
-    const int live = (sees + span - 1) / span;  // splits that hold a token it sees
-    const int64_t state = token_state(p, b, kv_head, token * p.group + head - kv_head * p.group, 0);
+    const int live = token_ceil(sees, span);  // splits that hold a token it sees
+    const int64_t state = token_state(p, first, kv_head, token * p.group + head - kv_head * p.group);
+    const int64_t next = token_state(p, 1, 0, 0);  // from one split's state to the next one's
     const float2* stats = reinterpret_cast<const float2*>(p.stats) + state;
     const float* numerator = p.numerator + state * D;
 
     float m = kNoToken;
     for (int s0 = 0; s0 < live; s0 += kWave) {
-        const float2 st = stats[imin(s0 + lane, live - 1)];
+        const float2 st = stats[imin(s0 + lane, live - 1) * next];
         m = fmaxf(m, st.y != 0.0f ? st.x : kNoToken);
     }
     m = wave_max(m);
     float l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = 0; s0 < live; s0 += kWave) {
-        const float2 st = stats[imin(s0 + lane, live - 1)];
+        const float2 st = stats[imin(s0 + lane, live - 1) * next];
         const float a = s0 + lane < live && st.y != 0.0f ? fast_exp2(st.x - m) : 0.0f;
         l += a != 0.0f ? st.y * a : 0.0f;
         const int here = imin(live - s0, kWave);
@@ -771,7 +836,7 @@ __global__ void __launch_bounds__(256) token_merge_kernel(const TokenParams p) {
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
                 const int at = imin(s0 + s + u * SPW + lane / LPS, live - 1);
-                x[u] = *reinterpret_cast<const f32x4*>(numerator + static_cast<int64_t>(at) * D + (lane % LPS) * 4);
+                x[u] = *reinterpret_cast<const f32x4*>(numerator + at * next * D + (lane % LPS) * 4);
             }
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {

@@ -29,7 +29,7 @@ int launch_tokens_format(const TokenParams& p, const TokenPlan& plan, hipStream_
     } else if constexpr (!(sizeof(QT) == 4 && D == 128)) {
         hipLaunchKernelGGL((token_kernel<QT, KVF, D, 2, 4, KT>), grid, dim3(4 * kWave), 0, stream, p);
     }
-    if (p.splits > 1) {
+    if (p.split != kTokenWhole) {
         const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens * p.query_heads;
         hipLaunchKernelGGL((token_merge_kernel<QT, D>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream, p);
     }

@@ -25,14 +25,15 @@ struct TokenParams {
     const int32_t* lengths;
     const int32_t* counts;   // or null: every token is live
     void* out;
-    float* numerator;        // [rows of all tiles, splits, D], splits > 1 only
-    float* stats;            // [rows of all tiles, splits, 2]
+    float* numerator;        // [items, kv_heads, rows of all tiles, D], where contexts are split
+    float* stats;            // [items, kv_heads, rows of all tiles, 2]
     int batch, tokens;
     int query_heads, kv_heads, group;
     int table_width, page_shift, physical_pages;
     int causal;
-    int splits;              // of each sequence's cache tokens
-    int split_tokens;        // tokens per split where `splits` of them reach the length
+    int split;               // how contexts are split: enum TokenSplit
+    int items;               // (sequence, split) pairs of the launch
+    int split_tokens;        // tokens per split, or more where the lengths outgrew what the host knew
     int tile_rows, row_tiles;
     int head_waves;          // stream kernel: KV heads of a workgroup
     uint32_t kv_row_bytes;   // bytes from one cache token to the next: kv_heads * D * element
@@ -55,55 +56,58 @@ PD_HD int token_sees(int causal, int context, int count, int j) {
     return causal ? imax(imin(context, context - count + j + 1), 0) : context;
 }
 
-// Tokens per split of a sequence: split_tokens, or more (a multiple of the
-// unit) where the context outgrew what the host knew.
+// Contexts are whole (item = sequence), or cut into splits of split_tokens
+// each. In a list, the sequences' splits follow one another, so that a short one
+// takes no more items than it has tokens for; the device works out the list from the
+// lengths, one lane a sequence (so up to kTokenListBatch of them), and takes longer splits where it
+// would not fit the items. Larger batches have the same number of splits in every sequence.
+enum TokenSplit { kTokenWhole = 0, kTokenList = 1, kTokenGrid = 2 };
+constexpr int kTokenListBatch = 64;
 constexpr int kTokenSplitUnit = 64;
 
-PD_HD int token_split(int splits, int split_tokens, int context) {
-    const int even = (context + splits - 1) / splits;
-    return imax(split_tokens, (even + kTokenSplitUnit - 1) / kTokenSplitUnit * kTokenSplitUnit);
+PD_HD int token_ceil(int a, int b) { return (a + b - 1) / b; }
+
+// Tokens per split of a sequence in a grid of `splits`: split_tokens, or more
+// (a multiple of the unit) where the context outgrew what the host knew.
+PD_HD int token_grid_span(int splits, int split_tokens, int context) {
+    return imax(split_tokens, token_ceil(token_ceil(context, splits), kTokenSplitUnit) * kTokenSplitUnit);
 }
 
 // Workgroup `block` of the launch (one grid dimension). Tiles that see most come
-// first, over all heads and splits, so that what remains at the end is short; a
-// (sequence, KV head, split) keeps its place modulo their number, so that with a multiple of
+// first, over all heads and items, so that what remains at the end is short; an
+// (item, KV head) keeps its place modulo their number, so that with a multiple of
 // eight of them its tiles, which read the same K and V, run on one XCD.
 struct TokenCoords {
-    int b, kv_head, split, tile;
+    int item, kv_head, tile;
 };
 
 PD_HD TokenCoords token_coords(const TokenParams& p, uint32_t block) {
-    const uint32_t units = static_cast<uint32_t>(p.batch * p.kv_heads * p.splits);
+    const uint32_t units = static_cast<uint32_t>(p.items * p.kv_heads);
     const uint32_t rank = block / units;
     const uint32_t unit = block - rank * units;
-    const uint32_t head = unit / p.splits;
     TokenCoords c;
     c.tile = p.row_tiles - 1 - static_cast<int>(rank);
-    c.split = static_cast<int>(unit - head * p.splits);
-    c.b = static_cast<int>(head / p.kv_heads);
-    c.kv_head = static_cast<int>(head - static_cast<uint32_t>(c.b) * p.kv_heads);
+    c.item = static_cast<int>(unit / p.kv_heads);
+    c.kv_head = static_cast<int>(unit - static_cast<uint32_t>(c.item) * p.kv_heads);
     return c;
 }
 
-// Stream kernel: workgroups of one split's KV heads are neighbours, wave w has
-// KV head w % head_waves of the workgroup's. Later splits, which short sequences
-// have nothing in, come last.
+// Stream kernel: workgroups of one item's KV heads are neighbours, wave w has KV
+// head w % head_waves of the workgroup's.
 PD_HD TokenCoords token_stream_coords(const TokenParams& p, uint32_t block, int wave) {
     const uint32_t head_groups = static_cast<uint32_t>(p.kv_heads / p.head_waves);
     const uint32_t unit = block / head_groups;
-    const uint32_t part = unit / p.row_tiles;
     TokenCoords c;
     c.kv_head = static_cast<int>(block - unit * head_groups) * p.head_waves + wave % p.head_waves;
-    c.tile = static_cast<int>(unit - part * p.row_tiles);
-    c.split = static_cast<int>(part / p.batch);
-    c.b = static_cast<int>(part - static_cast<uint32_t>(c.split) * p.batch);
+    c.item = static_cast<int>(unit / p.row_tiles);
+    c.tile = static_cast<int>(unit - static_cast<uint32_t>(c.item) * p.row_tiles);
     return c;
 }
 
-// State of row `row` (of the padded rows of all tiles) of (sequence, KV head) in split s.
-PD_HD int64_t token_state(const TokenParams& p, int b, int kv_head, int row, int s) {
+// State of row `row` (of the padded rows of all tiles) of (item, KV head).
+PD_HD int64_t token_state(const TokenParams& p, int item, int kv_head, int row) {
     const int64_t rows = static_cast<int64_t>(p.row_tiles) * p.tile_rows;
-    return ((static_cast<int64_t>(b) * p.kv_heads + kv_head) * rows + row) * p.splits + s;
+    return (static_cast<int64_t>(item) * p.kv_heads + kv_head) * rows + row;
 }
 
 // Element offset of row `row` of (sequence, KV head) in q and out.
@@ -113,19 +117,21 @@ PD_HD int64_t token_q_row(const TokenParams& p, int b, int kv_head, int token, i
 
 // 16-byte chunk position of chunk c of tile row r in LDS: chunks of a row are
 // permuted so that neither the reads of one chunk of many rows (K) nor those
-// of pairs of chunks of four rows (V, transposing) meet in a bank.
-template <int kRowBytes>
-PD_HD int token_chunk(int r, int c) {
-    if (kRowBytes == 128) return r * 8 + (c ^ ((((r >> 1) & 3) << 1) | ((r >> 3) & 1)));      // 16-bit, D 64
-    if (kRowBytes == 256) return r * 16 + (c ^ (((r & 7) << 1) | ((r >> 3) & 1)));            // 16-bit D 128, FP32 D 64
-    return r * 32 + (c ^ (r & 15));                                                          // FP32, D 128
+// of neighbouring rows that are transposed together (V: pairs of chunks of four rows;
+// FP8 as stored: one chunk of four rows and of those 16 behind) meet in a bank.
+// The permutation of a row is its own inverse.
+template <int kRowBytes, bool kFp8>
+PD_HD int token_slot_chunk(int r, int c) {
+    if (kRowBytes == 64) return c ^ (((r >> 2) ^ (r >> 4)) & 3);                                        // FP8, D 64
+    if (kRowBytes == 128 && kFp8) return c ^ ((((r >> 1) & 3) << 1) | (((r >> 3) ^ (r >> 4)) & 1));     // FP8, D 128
+    if (kRowBytes == 128) return c ^ ((((r >> 1) & 3) << 1) | ((r >> 3) & 1));                          // 16-bit, D 64
+    if (kRowBytes == 256) return c ^ (((r & 7) << 1) | ((r >> 3) & 1));                                 // 16-bit D 128, FP32 D 64
+    return c ^ (r & 15);                                                                                // FP32, D 128
 }
 
-// The chunk of row r that lies at position `slot` of the row's chunks: the
-// permutation is its own inverse.
-template <int kRowBytes>
-PD_HD int token_slot_chunk(int r, int slot) {
-    return token_chunk<kRowBytes>(r, slot) - r * (kRowBytes / 16);
+template <int kRowBytes, bool kFp8 = false>
+PD_HD int token_chunk(int r, int c) {
+    return r * (kRowBytes / 16) + token_slot_chunk<kRowBytes, kFp8>(r, c);
 }
 
 // ---------------------------------------------------------------------------
@@ -135,9 +141,9 @@ struct TokenPlan {
     bool stream;             // the kernel of few rows
     int tile_rows, row_tiles;
     int waves, head_waves;   // of a workgroup; stream kernel: KV heads among them
-    int splits, split_tokens;
+    int split, items, split_tokens;
     int64_t workgroups;
-    int64_t states;  // 0 with one split
+    int64_t states;  // 0 with whole contexts
 };
 
 constexpr int kStreamMaxRows = 32;     // rows that the stream kernel takes
@@ -145,21 +151,18 @@ constexpr int kStreamWaves = 8;        // waves of its workgroups (FP32 rows are
 constexpr int kTokenMinSplit = 128;    // cache tokens per split, at least
 constexpr int kTokenGroupsPerCu = 2;   // workgroups per CU that splits of the tile kernel aim at
 
-// The workgroups that a launch with splits of `span` tokens has anything to do in.
-inline int64_t live_splits(const int32_t* bounds, int batch, int64_t bound, int64_t span) {
-    if (bounds == nullptr) return batch * ((bound + span - 1) / span);
-    int64_t live = 0;
-    for (int b = 0; b < batch; ++b) live += (lmin(imax(bounds[b], 0), bound) + span - 1) / span;
-    return live;
+// Items of splits of `span` tokens.
+inline int64_t token_items(int split, const int32_t* bounds, int batch, int64_t bound, int64_t span) {
+    const int64_t most = (bound + span - 1) / span;
+    if (split == kTokenGrid || bounds == nullptr) return batch * most;
+    int64_t items = 0;
+    for (int b = 0; b < batch; ++b) items += (lmin(imax(bounds[b], 0), bound) + span - 1) / span;
+    return lmax(items, batch);
 }
 
-// Splits that `unsplit` workgroups are cut into at most: 1 if they fill the device.
-inline int64_t token_most_splits(int64_t unsplit, int64_t wanted) { return unsplit >= wanted ? 1 : 4 * wanted / unsplit; }
-
-// q_bytes: of a q element. bound: cache tokens the host knows no sequence to
-// exceed; bounds: and each of them (or null).
-inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads, int64_t bound,
-                             const int32_t* bounds, int64_t max_states, int compute_units) {
+// The launch without splits, and the workgroups that splits aim at.
+inline TokenPlan plan_whole_tokens(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads,
+                                   int compute_units, int64_t& wanted) {
     TokenPlan t{};
     const int64_t rows = static_cast<int64_t>(tokens) * (query_heads / kv_heads);
     t.stream = rows <= kStreamMaxRows;
@@ -173,46 +176,52 @@ inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, i
         t.head_waves = 1;
     }
     t.row_tiles = static_cast<int>((rows + t.tile_rows - 1) / t.tile_rows);
-    // Workgroups of one sequence's split, and how many the device should get.
-    const int64_t each = static_cast<int64_t>(kv_heads / t.head_waves) * t.row_tiles;
-    const int64_t wanted = static_cast<int64_t>(compute_units) * (t.stream ? 1 : kTokenGroupsPerCu);
-    const int64_t states = static_cast<int64_t>(batch) * kv_heads * t.row_tiles * t.tile_rows;  // of one split
-    // The shortest split with which the workgroups still fit the device at once; those that find nothing to do,
-    // a short sequence's in later splits, count a quarter.
-    const int64_t limit = lmin(token_most_splits(each * batch, wanted), max_states / states);
-    int64_t span = bound;
-    if (limit > 1) {
-        const int64_t least = lmax(kTokenMinSplit, (bound + limit - 1) / limit);
-        int64_t low = (least + kTokenSplitUnit - 1) / kTokenSplitUnit, high = (bound + kTokenSplitUnit - 1) / kTokenSplitUnit;
-        while (low < high) {  // units of tokens; more of them, fewer workgroups
-            const int64_t mid = (low + high) / 2;
-            if (each * live_splits(bounds, batch, bound, mid * kTokenSplitUnit) <= wanted) high = mid;
-            else low = mid + 1;
-        }
-        span = low * kTokenSplitUnit;
-    }
-    t.splits = static_cast<int>((bound + span - 1) / span);
-    t.split_tokens = t.splits > 1 ? static_cast<int>(span) : kTokenSplitUnit;
-    t.workgroups = each * batch * t.splits;
-    t.states = t.splits > 1 ? states * t.splits : 0;
+    t.split = kTokenWhole;
+    t.items = batch;
+    t.split_tokens = 1 << 30;
+    t.workgroups = static_cast<int64_t>(kv_heads / t.head_waves) * t.row_tiles * batch;
+    wanted = static_cast<int64_t>(compute_units) * (t.stream ? 1 : kTokenGroupsPerCu);
     return t;
 }
 
-// States with which no call of up to `tokens` tokens splits less than it would with
-// more: a split has at least kTokenMinSplit tokens, and unsplit calls at least `wanted` workgroups.
+// q_bytes: of a q element. bound: cache tokens the host knows no sequence to
+// exceed; bounds: and each of them (or null).
+inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads, int64_t bound,
+                             const int32_t* bounds, int64_t max_states, int compute_units) {
+    int64_t wanted;
+    TokenPlan t = plan_whole_tokens(q_bytes, head_dim, batch, tokens, query_heads, kv_heads, compute_units, wanted);
+    const int64_t each = t.workgroups / batch;  // workgroups of an item
+    const int64_t states = static_cast<int64_t>(kv_heads) * t.row_tiles * t.tile_rows;  // and its states
+    const int64_t limit = lmin(wanted / each, max_states / states);  // items that fit the device at once
+    if (t.workgroups >= wanted || limit <= batch) return t;
+    const int split = batch <= kTokenListBatch ? kTokenList : kTokenGrid;
+    // The shortest split with which the items fit; more tokens, fewer of them.
+    int64_t low = kTokenMinSplit / kTokenSplitUnit, high = (bound + kTokenSplitUnit - 1) / kTokenSplitUnit;
+    while (low < high) {
+        const int64_t mid = (low + high) / 2;
+        if (token_items(split, bounds, batch, bound, mid * kTokenSplitUnit) <= limit) high = mid;
+        else low = mid + 1;
+    }
+    const int64_t span = low * kTokenSplitUnit;
+    if (span >= bound) return t;
+    t.split = split;
+    t.split_tokens = static_cast<int>(span);
+    t.items = static_cast<int>(token_items(split, bounds, batch, bound, span));
+    t.workgroups = each * t.items;
+    t.states = states * t.items;
+    return t;
+}
+
+// States with which no call of up to `tokens` tokens splits less than it would with more.
 inline int64_t most_token_states(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads, int64_t reach,
                                  int compute_units) {
     int64_t most = 0;
-    for (int n = 1; n <= tokens; ++n) {
-        const TokenPlan t = plan_tokens(q_bytes, head_dim, batch, n, query_heads, kv_heads, reach, nullptr, 0, compute_units);
-        const int64_t wanted = static_cast<int64_t>(compute_units) * (t.stream ? 1 : kTokenGroupsPerCu);
-        if (t.workgroups >= wanted) {
-            if (t.stream) continue;
-            break;  // and so for every larger n
-        }
-        const int64_t splits = lmin(token_most_splits(t.workgroups, wanted), (reach + kTokenMinSplit - 1) / kTokenMinSplit);
-        const int64_t states = static_cast<int64_t>(batch) * kv_heads * t.row_tiles * t.tile_rows;
-        if (splits > 1 && splits * states > most) most = splits * states;
+    for (int n = 1; n <= tokens && reach > kTokenMinSplit; ++n) {
+        int64_t wanted;
+        const TokenPlan t = plan_whole_tokens(q_bytes, head_dim, batch, n, query_heads, kv_heads, compute_units, wanted);
+        if (t.workgroups >= wanted && !t.stream) break;  // and so for every larger n
+        const int64_t items = lmin(wanted / (t.workgroups / batch), batch * ((reach + kTokenMinSplit - 1) / kTokenMinSplit));
+        if (items > batch) most = lmax(most, items * kv_heads * t.row_tiles * t.tile_rows);
     }
     return most;
 }

@@ -100,7 +100,8 @@ int pd_decode_tokens(const void* q, int q_dtype, const void* k, const void* v, i
     p.page_shift = page_size == 16 ? 4 : 5;
     p.physical_pages = physical_pages;
     p.causal = causal != 0;
-    p.splits = plan.splits;
+    p.split = plan.split;
+    p.items = plan.items;
     p.split_tokens = plan.split_tokens;
     p.tile_rows = plan.tile_rows;
     p.row_tiles = plan.row_tiles;
