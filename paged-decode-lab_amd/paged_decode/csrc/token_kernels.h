@@ -542,7 +542,8 @@ __device__ __forceinline__ TokenItem token_item(const TokenParams& p, int item, 
 // sees a token of its split.
 template <int M>
 __device__ __forceinline__ bool open_work(const TokenParams& p, const TokenCoords& at, TokenWork& w, int& last, int lane) {
-    const TokenItem t = token_item(p, at.item, lane);
+    TokenItem t = token_item(p, imin(at.item, p.items - 1), lane);
+    if (at.item >= p.items) t.b = p.batch;
     w.b = imin(t.b, p.batch - 1);
     w.item = at.item;
     w.kv_head = at.kv_head;

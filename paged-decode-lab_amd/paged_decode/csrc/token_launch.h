@@ -15,7 +15,7 @@ int launch_tokens_bf16_d128(const TokenParams&, const TokenPlan&, int kv_dtype, 
 
 template <typename QT, int KVF, int D>
 int launch_tokens_format(const TokenParams& p, const TokenPlan& plan, hipStream_t stream) {
-    const dim3 grid(static_cast<uint32_t>(plan.workgroups));
+    const dim3 grid(static_cast<uint32_t>(token_workgroups(plan, p.kv_heads)));
     constexpr int KT = sizeof(QT) == 4 ? 32 : 64;
     if (plan.stream) {
         constexpr int WAVES = sizeof(QT) == 4 && D == 128 ? kStreamWaves / 2 : kStreamWaves;

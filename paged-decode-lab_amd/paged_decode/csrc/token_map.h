@@ -92,15 +92,22 @@ PD_HD TokenCoords token_coords(const TokenParams& p, uint32_t block) {
     return c;
 }
 
-// Stream kernel: workgroups of one item's KV heads are neighbours, wave w has KV
-// head w % head_waves of the workgroup's.
+// Stream kernel: wave w has KV head w % head_waves of the workgroup's. The
+// workgroups of one item's KV heads follow one another on one XCD (eight of
+// them, which take workgroups in turn), items in turn on the XCDs: heads in turn on them
+// would have an XCD read the same few hundred bytes of every token's row, a part of its L2's channels.
+// Items come in eights; those past the last one are empty.
+constexpr int kXcds = 8;
+
 PD_HD TokenCoords token_stream_coords(const TokenParams& p, uint32_t block, int wave) {
     const uint32_t head_groups = static_cast<uint32_t>(p.kv_heads / p.head_waves);
-    const uint32_t unit = block / head_groups;
+    const uint32_t slot = block / kXcds;
+    const uint32_t unit = slot / head_groups;
+    const uint32_t eight = unit / p.row_tiles;
     TokenCoords c;
-    c.kv_head = static_cast<int>(block - unit * head_groups) * p.head_waves + wave % p.head_waves;
-    c.item = static_cast<int>(unit / p.row_tiles);
-    c.tile = static_cast<int>(unit - static_cast<uint32_t>(c.item) * p.row_tiles);
+    c.kv_head = static_cast<int>(slot - unit * head_groups) * p.head_waves + wave % p.head_waves;
+    c.tile = static_cast<int>(unit - eight * p.row_tiles);
+    c.item = static_cast<int>(eight * kXcds + block % kXcds);
     return c;
 }
 
@@ -142,8 +149,8 @@ struct TokenPlan {
     int tile_rows, row_tiles;
     int waves, head_waves;   // of a workgroup; stream kernel: KV heads among them
     int split, items, split_tokens;
-    int64_t workgroups;
-    int64_t states;  // 0 with whole contexts
+    int64_t workgroups;  // with whole contexts
+    int64_t states;      // 0 with whole contexts
 };
 
 constexpr int kStreamMaxRows = 32;     // rows that the stream kernel takes
@@ -158,6 +165,12 @@ inline int64_t token_items(int split, const int32_t* bounds, int batch, int64_t 
     int64_t items = 0;
     for (int b = 0; b < batch; ++b) items += (lmin(imax(bounds[b], 0), bound) + span - 1) / span;
     return lmax(items, batch);
+}
+
+// Workgroups of a launch.
+inline int64_t token_workgroups(const TokenPlan& t, int kv_heads) {
+    if (!t.stream) return static_cast<int64_t>(t.items) * kv_heads * t.row_tiles;
+    return static_cast<int64_t>((t.items + kXcds - 1) / kXcds * kXcds) * (kv_heads / t.head_waves) * t.row_tiles;
 }
 
 // The launch without splits, and the workgroups that splits aim at.
@@ -192,8 +205,9 @@ inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, i
     TokenPlan t = plan_whole_tokens(q_bytes, head_dim, batch, tokens, query_heads, kv_heads, compute_units, wanted);
     const int64_t each = t.workgroups / batch;  // workgroups of an item
     const int64_t states = static_cast<int64_t>(kv_heads) * t.row_tiles * t.tile_rows;  // and its states
-    const int64_t limit = lmin(wanted / each, max_states / states);  // items that fit the device at once
-    if (t.workgroups >= wanted || limit <= batch) return t;
+    int64_t limit = lmin(wanted / each, max_states / states);  // items that fit the device at once
+    if (t.stream && limit > kXcds) limit -= limit % kXcds;     // and each of its XCDs
+    if (t.workgroups >= compute_units || limit <= batch) return t;
     const int split = batch <= kTokenListBatch ? kTokenList : kTokenGrid;
     // The shortest split with which the items fit; more tokens, fewer of them.
     int64_t low = kTokenMinSplit / kTokenSplitUnit, high = (bound + kTokenSplitUnit - 1) / kTokenSplitUnit;
@@ -207,7 +221,6 @@ inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, i
     t.split = split;
     t.split_tokens = static_cast<int>(span);
     t.items = static_cast<int>(token_items(split, bounds, batch, bound, span));
-    t.workgroups = each * t.items;
     t.states = states * t.items;
     return t;
 }
@@ -219,7 +232,7 @@ inline int64_t most_token_states(int q_bytes, int head_dim, int batch, int token
     for (int n = 1; n <= tokens && reach > kTokenMinSplit; ++n) {
         int64_t wanted;
         const TokenPlan t = plan_whole_tokens(q_bytes, head_dim, batch, n, query_heads, kv_heads, compute_units, wanted);
-        if (t.workgroups >= wanted && !t.stream) break;  // and so for every larger n
+        if (t.workgroups >= compute_units && !t.stream) break;  // and so for every larger n
         const int64_t items = lmin(wanted / (t.workgroups / batch), batch * ((reach + kTokenMinSplit - 1) / kTokenMinSplit));
         if (items > batch) most = lmax(most, items * kv_heads * t.row_tiles * t.tile_rows);
     }
