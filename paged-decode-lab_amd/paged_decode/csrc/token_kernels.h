@@ -502,13 +502,14 @@ struct TokenItem {
     int span;
 };
 
-// Sums of x over lanes 0 .. lane.
-__device__ __forceinline__ int wave_prefix(int x, int lane) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const int y = __shfl_up(x, d);
-        x += lane >= d ? y : 0;
-    }
+// Sums of x over lanes 0 .. lane: within each row of 16 lanes, then the last lanes' of the rows before.
+__device__ __forceinline__ int wave_prefix(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // row_shr 1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15: into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast 31: into rows 2 and 3
     return x;
 }
 
@@ -517,7 +518,7 @@ __device__ __forceinline__ int wave_prefix(int x, int lane) {
 __device__ __forceinline__ int token_list(const TokenParams& p, int lane, int& span) {
     const int context = lane < p.batch ? token_context(p, lane) : 0;
     for (span = p.split_tokens;; span *= 2) {  // ends: with one split each there are no more than sequences
-        const int upto = wave_prefix(token_ceil(context, span), lane);
+        const int upto = wave_prefix(token_ceil(context, span));
         if (__builtin_amdgcn_readlane(upto, kWave - 1) <= p.items) return upto;
     }
 }
@@ -754,50 +755,71 @@ __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const Token
         if (quad == 0) states[wave][r * 16 + col] = make_float2(rows.m[r], sum);
     }
     __syncthreads();
-    constexpr int PER = D / kWave;
-    for (int i = slice; i < M; i += slices) {
+    // Four dims of a row a lane; all waves of the head together, and a few states' reads at once.
+    constexpr int LPR = D / 4, RPW = kWave / LPR;  // lanes per row, rows per wave
+    constexpr int kAtOnce = WAVES / 2;             // divides the slices of either number of heads per workgroup
+    const int dim = (lane % LPR) * 4;
+    const int mate = wave % late.head_waves;       // the first wave of the same head
+    for (int i = slice * RPW + lane / LPR; i < M; i += slices * RPW) {
         const int row = w.row0 + i, token = row / late.group;
-        if (token >= late.tokens) break;
-        float m = kNoToken, l = 0.0f, o[PER];
-        for (int j = wave % late.head_waves; j < WAVES; j += late.head_waves)
-            if (states[j][i].y != 0.0f) m = fmaxf(m, states[j][i].x);
+        if (token >= late.tokens) continue;
+        float m = kNoToken, l = 0.0f;
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j0 = 0; j0 < slices; j0 += kAtOnce)
 #pragma unroll
-        for (int e = 0; e < PER; ++e) o[e] = 0.0f;
-        for (int j = wave % late.head_waves; j < WAVES; j += late.head_waves) {
-            const float2 st = states[j][i];
-            const float a = st.y != 0.0f ? fast_exp2(st.x - m) : 0.0f;
-            l += st.y * a;
-            const float* from = reinterpret_cast<const float*>(regions + j * Shape::REGION) + i * Shape::SD + lane * PER;
+            for (int j = 0; j < kAtOnce; ++j) {
+                const float2 st = states[mate + (j0 + j) * late.head_waves][i];
+                m = fmaxf(m, st.y != 0.0f ? st.x : kNoToken);
+            }
+        for (int j0 = 0; j0 < slices; j0 += kAtOnce) {
+            f32x4 x[kAtOnce];
+            float a[kAtOnce];
 #pragma unroll
-            for (int e = 0; e < PER; ++e) o[e] = fmaf(from[e], a, o[e]);
+            for (int j = 0; j < kAtOnce; ++j) {
+                const int from = mate + (j0 + j) * late.head_waves;
+                const float2 st = states[from][i];
+                a[j] = st.y != 0.0f ? fast_exp2(st.x - m) : 0.0f;
+                l = fmaf(st.y, a[j], l);
+                x[j] = *reinterpret_cast<const f32x4*>(regions + from * Shape::REGION + (i * Shape::SD + dim) * 4);
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(x[j][e], a[j], o[e]);
         }
         if (late.split == kTokenWhole) {
-            QT* out = static_cast<QT*>(late.out) + token_q_row(late, w.b, w.kv_head, token, row - token * late.group) * D + lane * PER;
+            QT* out = static_cast<QT*>(late.out) + token_q_row(late, w.b, w.kv_head, token, row - token * late.group) * D + dim;
             const float inv = l == 0.0f ? 0.0f : late.v_scale / l;
 #pragma unroll
-            for (int e = 0; e < PER; ++e) out[e] = static_cast<QT>(l == 0.0f ? 0.0f : o[e] * inv);
+            for (int e = 0; e < 4; ++e) o[e] = l == 0.0f ? 0.0f : o[e] * inv;
+            if constexpr (Rows::kF32) *reinterpret_cast<f32x4*>(out) = o;
+            else
+                *reinterpret_cast<u32x2*>(out) = u32x2{Rows::Math::pack(o[0], o[1]), Rows::Math::pack(o[2], o[3])};
         } else if (row < w.rows) {
             const int64_t state = token_state(late, w.item, w.kv_head, row);
-#pragma unroll
-            for (int e = 0; e < PER; ++e) late.numerator[state * D + lane * PER + e] = o[e] * late.v_scale;
-            if (lane == 0) *reinterpret_cast<float2*>(late.stats + state * 2) = make_float2(m, l);
+            *reinterpret_cast<f32x4*>(late.numerator + state * D + dim) = o * late.v_scale;
+            if (dim == 0) *reinterpret_cast<float2*>(late.stats + state * 2) = make_float2(m, l);
         }
     }
 }
 
 // ---------------------------------------------------------------------------
-// Splits of each row into its output: a wave per row, four dims a lane, so that
-// kWave / (D / 4) states are read at once, kUnroll times over before the first is used:
-// a row's reads are what the kernel waits for.
-template <typename QT, int D>
+// Splits of each row into its output: kWaves waves per row (1 or 4), which take
+// parts of its splits. Four dims a lane, so that kWave / (D / 4) states are read
+// at once, kUnroll times over and together with the statistics: a row's reads, of
+// lengths, then of states, are what the kernel waits for.
+template <typename QT, int D, int kWaves>
 __global__ void __launch_bounds__(256) token_merge_kernel(const TokenParams p) {
     constexpr int LPS = D / 4;          // lanes per state
     constexpr int SPW = kWave / LPS;    // states per read
-    constexpr int kUnroll = 4;
+    constexpr int kUnroll = 16 / SPW;   // reads of 16 states
+    __shared__ f32x4 sums[kWaves][LPS];
+    __shared__ float2 parts[kWaves];
     const int lane = threadIdx.x % kWave;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * (4 / kWaves) + wave / kWaves;
     const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens * p.query_heads;
-    if (item >= rows) return;
+    if (item >= rows) return;  // with several waves per row, all of a workgroup or none
     const uint32_t bt = static_cast<uint32_t>(item / p.query_heads);
     const int head = static_cast<int>(item - static_cast<int64_t>(bt) * p.query_heads);
     const int b = static_cast<int>(bt / p.tokens), token = static_cast<int>(bt - static_cast<uint32_t>(b) * p.tokens);
@@ -813,32 +835,38 @@ __global__ void __launch_bounds__(256) token_merge_kernel(const TokenParams p) {
     }
     const int count = token_count(p, b), context = token_context(p, b);
     const int sees = token < count ? token_sees(p.causal, context, count, token) : 0;
-    const int live = token_ceil(sees, span);  // splits that hold a token it sees
-    const int64_t state = token_state(p, first, kv_head, token * p.group + head - kv_head * p.group);
+    const int all = token_ceil(sees, span);  // splits that hold a token it sees
     const int64_t next = token_state(p, 1, 0, 0);  // from one split's state to the next one's
+    const int share = token_ceil(all, kWaves), from0 = (wave % kWaves) * share;
+    const int live = imin(all - from0, share);     // this wave's, from from0 on
+    const int64_t state = token_state(p, first, kv_head, token * p.group + head - kv_head * p.group) + from0 * next;
     const float2* stats = reinterpret_cast<const float2*>(p.stats) + state;
-    const float* numerator = p.numerator + state * D;
+    const float* numerator = p.numerator + state * D + (lane % LPS) * 4;
 
-    float m = kNoToken;
-    for (int s0 = 0; s0 < live; s0 += kWave) {
-        const float2 st = stats[imin(s0 + lane, live - 1) * next];
-        m = fmaxf(m, st.y != 0.0f ? st.x : kNoToken);
-    }
-    m = wave_max(m);
-    float l = 0.0f;
+    float m = kNoToken, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = 0; s0 < live; s0 += kWave) {
-        const float2 st = stats[imin(s0 + lane, live - 1) * next];
-        const float a = s0 + lane < live && st.y != 0.0f ? fast_exp2(st.x - m) : 0.0f;
-        l += a != 0.0f ? st.y * a : 0.0f;
         const int here = imin(live - s0, kWave);
-        for (int s = 0; s < here; s += SPW * kUnroll) {
-            f32x4 x[kUnroll];
+        f32x4 x[kUnroll];
+        auto read = [&](int s) {
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
-                const int at = imin(s0 + s + u * SPW + lane / LPS, live - 1);
-                x[u] = *reinterpret_cast<const f32x4*>(numerator + at * next * D + (lane % LPS) * 4);
+                const int at = s0 + imin(s + u * SPW + lane / LPS, here - 1);
+                x[u] = *reinterpret_cast<const f32x4*>(numerator + at * next * D);
             }
+        };
+        const float2 st = stats[(s0 + imin(lane, here - 1)) * next];
+        read(0);
+        const bool filled = lane < here && st.y != 0.0f;
+        const float top = fmaxf(m, wave_max(filled ? st.x : kNoToken));
+        const float alpha = fast_exp2(m - top);  // of the 64 splits before
+        m = top;
+        const float a = filled ? fast_exp2(st.x - m) : 0.0f;
+        l = fmaf(l, alpha, filled ? st.y * a : 0.0f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = alpha != 0.0f ? o[e] * alpha : 0.0f;
+        for (int s = 0; s < here; s += SPW * kUnroll) {
+            if (s > 0) read(s);
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
                 const int from = s + u * SPW + lane / LPS;
@@ -854,6 +882,25 @@ __global__ void __launch_bounds__(256) token_merge_kernel(const TokenParams p) {
     for (int e = 0; e < 4; ++e) {
         if constexpr (LPS == 16) o[e] += __shfl_xor(o[e], 16);
         o[e] += __shfl_xor(o[e], 32);
+    }
+    if constexpr (kWaves > 1) {
+        if (lane < LPS) sums[wave][lane] = o;
+        if (lane == 0) parts[wave] = make_float2(m, l);
+        __syncthreads();
+        if (wave > 0) return;
+        float top = kNoToken;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) top = fmaxf(top, parts[i].y != 0.0f ? parts[i].x : kNoToken);
+        l = 0.0f;
+        o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            const float a = parts[i].y != 0.0f ? fast_exp2(parts[i].x - top) : 0.0f;
+            l = fmaf(parts[i].y, a, l);
+            const f32x4 x = sums[i][lane % LPS];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = a != 0.0f ? fmaf(x[e], a, o[e]) : o[e];
+        }
     }
     if (lane < LPS) {
         QT* out = static_cast<QT*>(p.out) + item * D + lane * 4;

@@ -13,6 +13,9 @@ int launch_tokens_f16_d128(const TokenParams&, const TokenPlan&, int kv_dtype, h
 int launch_tokens_bf16_d64(const TokenParams&, const TokenPlan&, int kv_dtype, hipStream_t);
 int launch_tokens_bf16_d128(const TokenParams&, const TokenPlan&, int kv_dtype, hipStream_t);
 
+// Splits of a sequence, on average, up to which a wave merges a row.
+constexpr int kMergeWaveSplits = 12;
+
 template <typename QT, int KVF, int D>
 int launch_tokens_format(const TokenParams& p, const TokenPlan& plan, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(token_workgroups(plan, p.kv_heads)));
@@ -31,7 +34,12 @@ int launch_tokens_format(const TokenParams& p, const TokenPlan& plan, hipStream_
     }
     if (p.split != kTokenWhole) {
         const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens * p.query_heads;
-        hipLaunchKernelGGL((token_merge_kernel<QT, D>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream, p);
+        // Four waves for a row of many splits, where one would read them in turns.
+        if (p.items > kMergeWaveSplits * p.batch) {
+            hipLaunchKernelGGL((token_merge_kernel<QT, D, 4>), dim3(static_cast<uint32_t>(rows)), dim3(256), 0, stream, p);
+        } else {
+            hipLaunchKernelGGL((token_merge_kernel<QT, D, 1>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream, p);
+        }
     }
     return hipGetLastError() == hipSuccess ? PD_OK : PD_ERR_LAUNCH;
 }
