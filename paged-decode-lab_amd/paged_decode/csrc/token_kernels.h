@@ -27,7 +27,6 @@ struct TokenMath;
 
 template <>
 struct TokenMath<_Float16> {
-    typedef f16x8 Frag;
     // Weights lie below 2^14 and the running maximum's own at 2^6, so that those 2^-20 of it keep 11 bits.
     static constexpr float kOffset = 6.0f, kSlack = 14.0f;
     static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
@@ -49,11 +48,11 @@ struct TokenMath<_Float16> {
         return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
     }
     static constexpr uint32_t kExponents = 0x7C007C00u, kLast = 0x04000400u;  // and their last bits
+    static constexpr uint32_t kOnes = 0x3C003C00u;                                     // 1.0 twice
 };
 
 template <>
 struct TokenMath<__bf16> {
-    typedef bf16x8 Frag;
     static constexpr float kOffset = 0.0f, kSlack = 8.0f;
     static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -74,6 +73,7 @@ struct TokenMath<__bf16> {
         return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
     }
     static constexpr uint32_t kExponents = 0x7F807F80u, kLast = 0x00800080u;  // and their last bits
+    static constexpr uint32_t kOnes = 0x3F803F80u;                                     // 1.0 twice
 };
 
 template <>
@@ -107,20 +107,30 @@ __device__ __forceinline__ float stored_value(const char* p, int i) {
     return f[0];
 }
 
+// Address of an LDS array within the workgroup's LDS.
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p));
+}
+
+template <typename T>
+__device__ __forceinline__ T lds_read(uint32_t at) {
+    return *(const __attribute__((address_space(3))) T*)at;
+}
+
 // Eight bytes of LDS per lane, transposed among each 16 lanes: these address
 // four rows of 16 16-bit elements (lane i: row i / 4, elements 4 (i % 4) on), and
 // lane i gets element i of each row.
-__device__ __forceinline__ u32x2 transposed_read(const char* p) {
+__device__ __forceinline__ u32x2 transposed_read(uint32_t at) {
     typedef __attribute__((address_space(3))) s16x4 LdsVec;
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec*)p));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec*)at));
 }
 
 // The same of bytes: each 16 lanes address eight rows of 16 bytes (lane i: row
 // i / 2, bytes 8 (i % 2) on), and lane i gets byte i of each row.
-__device__ __forceinline__ u32x2 transposed_bytes(const char* p) {
+__device__ __forceinline__ u32x2 transposed_bytes(uint32_t at) {
     typedef int i32x2 __attribute__((ext_vector_type(2)));
     typedef __attribute__((address_space(3))) i32x2 LdsVec;
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsVec*)p));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsVec*)at));
 }
 
 // What a workgroup of the kernel works on.
@@ -207,11 +217,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const char* base, u
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, 0x00027000);
 }
 
-// Address of an LDS array within the workgroup's LDS.
-__device__ __forceinline__ uint32_t lds_address(const char* p) {
-    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p));
-}
-
 // 16 bytes per lane from a buffer into LDS at to + kOffset + 16 lane, past the
 // registers. In assembly since the compiler, where it knows of such a load, waits for it
 // before the next read of any LDS; here wait_for_loads and a barrier come
@@ -259,15 +264,17 @@ struct TileLoad {
     static constexpr int RB = kWiden ? D * static_cast<int>(sizeof(QT)) : SB;           // and in LDS
     static constexpr int RPI = 1024 / SB;                        // rows per request of a wave
     static constexpr int NL = KT * SB / 1024 / WAVES;            // requests per wave
+    static constexpr int RPW = RPI * NL;                         // neighbouring rows, of 16 or of part of 16 if they are few
     static constexpr int LPR = SB / 16;                          // lanes per row
     static_assert(NL * WAVES * 1024 == KT * SB && 16 % RPI == 0, "whole requests, within 16 tokens");
+    static_assert(16 % RPW == 0 || RPW % 16 == 0, "whole blocks of 16 tokens, or parts of one");
     static_assert(!kWiden || kFp8, "what is widened");
     u32x4 raw[kWiden ? NL : 1];
 
     // ids: tile_pages of the tile; head: the cache from its KV head on; to: the tile's address in LDS.
     __device__ __forceinline__ void request(const TokenParams& p, int ids, const char* head, uint32_t to, int t0, int end,
                                             int wave, int lane) {
-        request_part(std::make_integer_sequence<int, NL>{}, p, ids, head, to + wave * (RPI * RB), t0, end, wave, lane);
+        request_part(std::make_integer_sequence<int, NL>{}, p, ids, head, to + wave * (RPW * RB), t0, end, wave, lane);
     }
 
     template <int... kParts>
@@ -279,17 +286,16 @@ struct TileLoad {
     template <int kPart>
     __device__ __forceinline__ void request_one(const TokenParams& p, int ids, const char* head, uint32_t to, int t0, int end,
                                                 int wave, int lane) {
-        const int row0 = RPI * (wave + WAVES * kPart);
-        const int block = row0 / 16;
+        const int block = wave * RPW / 16 + kPart * RPI / 16;
         const RowBlock rows = row_block(p, __builtin_amdgcn_readlane(ids, block), t0 + 16 * block, end);
-        const int r = row0 % 16 + lane / LPR;
+        const int r = wave * RPW % 16 + kPart * RPI % 16 + lane / LPR;
         if constexpr (kWiden) {
             const uint32_t offset = r * p.kv_row_bytes + (lane % LPR) * 16;
             raw[kPart] = __builtin_amdgcn_raw_buffer_load_b128(row_buffer(head + rows.offset, rows.bytes), offset, 0, 0);
         } else {
             // LDS slot `lane` of the request holds the chunk that token_chunk puts there.
-            const uint32_t offset = r * p.kv_row_bytes + token_slot_chunk<RB, kFp8>(row0 + lane / LPR, lane % LPR) * 16;
-            load_to_lds<kPart * WAVES * RPI * RB>(head + rows.offset, rows.bytes, to, offset);
+            const uint32_t offset = r * p.kv_row_bytes + token_slot_chunk<RB, kFp8>(16 * block + r, lane % LPR) * 16;
+            load_to_lds<kPart * RPI * RB>(head + rows.offset, rows.bytes, to, offset);
         }
     }
 
@@ -297,7 +303,7 @@ struct TileLoad {
         if constexpr (kWiden) {
 #pragma unroll
             for (int jj = 0; jj < NL; ++jj) {
-                const int r = RPI * (wave + WAVES * jj) + lane / LPR;
+                const int r = RPW * wave + RPI * jj + lane / LPR;
                 const u32x4 w = raw[jj];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -329,7 +335,8 @@ struct TokenRowsState {
     using Math = TokenMath<QT>;
     u32x4 q[R][KS];
     f32x4 o[R][ND];
-    float m[R], l[R];
+    f32x4 l[R];              // sums of weights: all four the whole one (FP32: of the lane's tokens 4 i + e)
+    float m[R], most[R];     // scores count from m on, and raise it where they lie above most
     int sees[R];
 
     __device__ __forceinline__ void open(const TokenParams& p, const TokenWork& w, int first_row, int lane) {
@@ -348,17 +355,38 @@ struct TokenRowsState {
                                                               token_q_row(p, w.b, w.kv_head, token, row - token * p.group) * D +
                                                               (4 * s + quad) * CE);
             }
-            m[r] = kNoToken;
-            l[r] = 0.0f;
+            m[r] = 0.0f;
+            most[r] = -INFINITY;  // the first token seen sets m
+            l[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[r][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
 
+    // Where the lane reads in a tile at `tile` in LDS: bases that constants are added to from one block of tokens to the next.
+    // FP8 as stored: rows 16 behind lie in other chunks.
+    __device__ __forceinline__ uint32_t k_base(uint32_t tile, int ks, int odd, int lane) const {
+        const int col = lane % 16, quad = lane / 16;
+        if constexpr (kFp8) return tile + (token_chunk<RB, true>(16 * odd + col, 2 * ks + quad / 2) - odd * RB) * 16 + (quad % 2) * 8;
+        else return tile + token_chunk<RB>(col, 4 * ks + quad) * 16;
+    }
+
+    // Dim 16 d + col of tokens 4 quad .. + 3 and of those 16 behind, by transposing reads: the 16 lanes of a quad address four
+    // rows of four 8-byte pieces (FP8: all eight rows).
+    __device__ __forceinline__ uint32_t v_base(uint32_t tile, int d, int lane) const {
+        const int col = lane % 16, quad = lane / 16;
+        if constexpr (kFp8) return tile + token_chunk<RB, true>(4 * quad + (col / 2) % 4 + (col / 8) * 16, d) * 16 + (col % 2) * 8;
+        else return tile + token_chunk<RB>(4 * quad + col / 4, 2 * d + (col % 4) / 2) * 16 + (col % 2) * 8;
+    }
+
     // Scores of a tile of 16 NI tokens, transposed: lane (col, quad) holds row col, tokens 16 i + 4 quad + e.
     template <int NI>
-    __device__ __forceinline__ void score(const char* k_tile, f32x4 (&s)[R][NI], int lane) {
-        const int col = lane % 16, quad = lane / 16;
+    __device__ __forceinline__ void score(uint32_t k_tile, f32x4 (&s)[R][NI], int lane) {
+        uint32_t base[kFp8 ? 2 : 1][KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int odd = 0; odd < (kFp8 ? 2 : 1); ++odd) base[odd][ks] = k_base(k_tile, ks, odd, lane);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
 #pragma unroll
@@ -367,12 +395,11 @@ struct TokenRowsState {
             for (int ks = 0; ks < KS; ++ks) {
                 u32x4 kf;
                 if constexpr (kFp8) {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(
-                        k_tile + token_chunk<RB, true>(16 * i + col, 2 * ks + quad / 2) * 16 + (quad % 2) * 8);
+                    const u32x2 w = lds_read<u32x2>(base[i % 2][ks] + i * 16 * RB);
                     const u32x2 a = Math::template widen<KVF>(w[0]), b = Math::template widen<KVF>(w[1]);
                     kf = u32x4{a[0], a[1], b[0], b[1]};
                 } else {
-                    kf = *reinterpret_cast<const u32x4*>(k_tile + token_chunk<RB>(16 * i + col, 4 * ks + quad) * 16);
+                    kf = lds_read<u32x4>(base[0][ks] + i * 16 * RB);
                 }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
@@ -388,15 +415,19 @@ struct TokenRowsState {
         }
     }
 
-    // Their weights, and the running maximum and sum. t0: the tile's first token; masked (uniform): some row does not see
-    // some token of it.
+    // Their weights, and the running maximum. t0: the tile's first token; masked (uniform): some row does not see some token of
+    // it. The largest exponent is looked for after the scaling, whose results the maximum takes as they are.
     template <int NI>
     __device__ __forceinline__ void weigh(f32x4 (&s)[R][NI], int t0, bool masked, uint32_t invalid, float scale_log2, int lane) {
         const int quad = lane / 16;
-        float most[R];  // of the lane's own scores
+        float top[R];  // of the lane's own
         bool grow = false;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[r][i][e] = fmaf(s[r][i][e], scale_log2, -m[r]);
             if (masked) {
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
@@ -406,54 +437,62 @@ struct TokenRowsState {
                         s[r][i][e] = seen ? s[r][i][e] : -INFINITY;
                     }
             }
-            most[r] = s[r][0][0];
+            top[r] = -INFINITY;
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) most[r] = fmaxf(most[r], s[r][i][e]);
-            grow |= most[r] * scale_log2 > m[r] + Math::kSlack;
+                for (int e = 0; e < 4; ++e) top[r] = fmaxf(top[r], s[r][i][e]);
+            grow |= top[r] > most[r];
         }
         if (__any(grow)) {  // only then do a row's four lanes compare
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const float top = max_over_lane_groups(most[r]) * scale_log2;
-                const float next = top > m[r] + Math::kSlack ? top - Math::kOffset : m[r];
-                const float alpha = fast_exp2(m[r] - next);
-                m[r] = next;
+                const float row_top = max_over_lane_groups(top[r]);
+                const bool above = row_top > most[r];
+                const float up = above ? row_top - Math::kOffset : 0.0f;
+                const float alpha = fast_exp2(fminf(-up, 0.0f));  // the first time up may be below 0, with sums of 0 as yet
+                most[r] = above ? Math::kSlack : most[r];
+                m[r] += up;
                 l[r] *= alpha;
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[r][d] *= alpha;
+#pragma unroll
+                for (int i = 0; i < NI; ++i) s[r][i] -= up;
             }
         }
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
+            for (int i = 0; i < NI; ++i) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[r][i][e] = fast_exp2(fmaf(s[r][i][e], scale_log2, -m[r]));
-                    l[r] += s[r][i][e];
-                }
+                for (int e = 0; e < 4; ++e) s[r][i][e] = fast_exp2(s[r][i][e]);
+                if constexpr (kF32) l[r] += s[r][i];
+            }
     }
 
-    // o^T += V^T w^T, 32 tokens a step (FP32: four).
+    // o^T += V^T w^T and l += 1^T w^T, 32 tokens a step (FP32: four, and l on the vector units).
     template <int NI>
-    __device__ __forceinline__ void add(const char* v_tile, const f32x4 (&s)[R][NI], int lane) {
-        const int col = lane % 16, quad = lane / 16;
+    __device__ __forceinline__ void add(uint32_t v_tile, const f32x4 (&s)[R][NI], int lane) {
         if constexpr (kF32) {
+            const int col = lane % 16, quad = lane / 16;
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        const float vf = *reinterpret_cast<const float*>(
-                            v_tile + token_chunk<RB>(16 * i + 4 * quad + e, 4 * d + col / 4) * 16 + (col % 4) * 4);
+                    for (int h = 0; h < ND / 4; ++h) {  // four dims a lane: those of a piece()
+                        const f32x4 vf = lds_read<f32x4>(v_tile + token_chunk<RB>(4 * quad + e, 16 * h + col) * 16 + i * 16 * RB);
 #pragma unroll
-                        for (int r = 0; r < R; ++r)
-                            o[r][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, s[r][i][e], o[r][d], 0, 0, 0);
+                        for (int d = 0; d < 4; ++d)
+#pragma unroll
+                            for (int r = 0; r < R; ++r)
+                                o[r][4 * h + d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[d], s[r][i][e], o[r][4 * h + d], 0, 0, 0);
                     }
         } else {
+            constexpr u32x4 ones = {Math::kOnes, Math::kOnes, Math::kOnes, Math::kOnes};
+            uint32_t base[ND];
+#pragma unroll
+            for (int d = 0; d < ND; ++d) base[d] = v_base(v_tile, d, lane);
 #pragma unroll
             for (int u = 0; u < NI / 2; ++u) {
                 u32x4 wt[R];
@@ -461,22 +500,18 @@ struct TokenRowsState {
                 for (int r = 0; r < R; ++r) {
                     const f32x4 a = s[r][2 * u], b = s[r][2 * u + 1];
                     wt[r] = u32x4{Math::pack(a[0], a[1]), Math::pack(a[2], a[3]), Math::pack(b[0], b[1]), Math::pack(b[2], b[3])};
+                    l[r] = Math::mma(ones, wt[r], l[r]);
                 }
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    // Lane (col, quad) gets dim 16 d + col of tokens 4 quad .. + 3 and of those 16 behind, by transposing
-                    // reads: the 16 lanes of a quad address four rows of four 8-byte pieces (FP8: all eight rows).
                     u32x4 vf;
                     if constexpr (kFp8) {
-                        const int row = 32 * u + 4 * quad + (col / 2) % 4 + (col / 8) * 16;
-                        const u32x2 w = transposed_bytes(v_tile + token_chunk<RB, true>(row, d) * 16 + (col % 2) * 8);
+                        const u32x2 w = transposed_bytes(base[d] + u * 32 * RB);
                         const u32x2 a = Math::template widen<KVF>(w[0]), b = Math::template widen<KVF>(w[1]);
                         vf = u32x4{a[0], a[1], b[0], b[1]};
                     } else {
-                        const int row = 32 * u + 4 * quad + col / 4;
-                        const int piece = 2 * d + (col % 4) / 2;
-                        const u32x2 v0 = transposed_read(v_tile + token_chunk<RB>(row, piece) * 16 + (col % 2) * 8);
-                        const u32x2 v1 = transposed_read(v_tile + token_chunk<RB>(row + 16, piece) * 16 + (col % 2) * 8);
+                        const u32x2 v0 = transposed_read(base[d] + u * 32 * RB);
+                        const u32x2 v1 = transposed_read(base[d] + u * 32 * RB + 16 * RB);
                         vf = u32x4{v0[0], v0[1], v1[0], v1[1]};
                     }
 #pragma unroll
@@ -484,6 +519,26 @@ struct TokenRowsState {
                 }
             }
         }
+    }
+
+    // Four neighbouring dims of o, and which: piece 0 .. ND - 1 of the lane's row. FP32 V is read four dims at once, so that a
+    // block's dims there are every fourth one.
+    __device__ __forceinline__ f32x4 piece(int r, int i) const {
+        if constexpr (kF32) {
+            const int h = i / 4 * 4, e = i % 4;
+            return f32x4{o[r][h][e], o[r][h + 1][e], o[r][h + 2][e], o[r][h + 3][e]};
+        } else {
+            return o[r][i];
+        }
+    }
+    static __device__ __forceinline__ int piece_dim(int i, int lane) {
+        return kF32 ? i / 4 * 64 + lane / 16 * 16 + i % 4 * 4 : 16 * i + lane / 16 * 4;
+    }
+
+    // A row's sum of weights, in all of its lanes.
+    __device__ __forceinline__ float sum(int r) const {
+        if constexpr (kF32) return sum_over_lane_groups((l[r][0] + l[r][1]) + (l[r][2] + l[r][3]));
+        else return l[r][0];
     }
 };
 
@@ -598,6 +653,7 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
     rows.open(p, w, w.row0 + wave * R * 16, lane);
 
     int buffer = 0;
+    bool one_by_one = false;
     for (int t0 = w.begin; t0 < w.end; t0 += KT, buffer ^= 1) {
         char* k_tile = k_tiles + buffer * TILE;
         char* v_tile = v_tiles + buffer * TILE;
@@ -615,23 +671,27 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
             bool bad = false;
             for (int i = threadIdx.x; i < TILE / 16; i += WAVES * kWave)
                 bad |= holds_nonfinite<QT, kTokenNative>(*reinterpret_cast<const u32x4*>(v_tile + i * 16));
-            if (__syncthreads_or(bad)) {
-                wait_for_loads();
-                token_rows_one_by_one<QT, KVF, D>(p, w, M, wave, WAVES, lane);
-                return;
+            bad = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad));  // known to be uniform: the loop's state stays in place
+            if (bad) {
+                one_by_one = true;
+                break;
             }
         }
         f32x4 s[R][KT / 16];
-        rows.score(k_tile, s, lane);
+        rows.score(k_at + buffer * TILE, s, lane);
         rows.weigh(s, t0, t0 + KT > common || here != 0 || partial, here, p.scale_log2, lane);
-        rows.add(v_tile, s, lane);
+        rows.add(v_at + buffer * TILE, s, lane);
     }
     wait_for_loads();  // the last request's: nothing may write LDS behind the workgroup's end
+    if (one_by_one) {
+        token_rows_one_by_one<QT, KVF, D>(p, w, M, wave, WAVES, lane);
+        return;
+    }
 
     const int col = lane % 16, quad = lane / 16;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const float sum = sum_over_lane_groups(rows.l[r]);
+        const float sum = rows.sum(r);
         const int row = w.row0 + (wave * R + r) * 16 + col;
         const int token = row / p.group;
         if (p.split == kTokenWhole) {
@@ -640,19 +700,19 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
             QT* out = static_cast<QT*>(p.out) + token_q_row(p, w.b, w.kv_head, token, row - token * p.group) * D;
 #pragma unroll
             for (int d = 0; d < Rows::ND; ++d) {
-                f32x4 x;
+                f32x4 x = rows.piece(r, d);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = sum == 0.0f ? 0.0f : rows.o[r][d][e] * inv;
-                if constexpr (Rows::kF32) *reinterpret_cast<f32x4*>(out + 16 * d + 4 * quad) = x;
+                for (int e = 0; e < 4; ++e) x[e] = sum == 0.0f ? 0.0f : x[e] * inv;
+                if constexpr (Rows::kF32) *reinterpret_cast<f32x4*>(out + rows.piece_dim(d, lane)) = x;
                 else
-                    *reinterpret_cast<u32x2*>(out + 16 * d + 4 * quad) =
+                    *reinterpret_cast<u32x2*>(out + rows.piece_dim(d, lane)) =
                         u32x2{Rows::Math::pack(x[0], x[1]), Rows::Math::pack(x[2], x[3])};
             }
         } else if (row < w.rows) {
             const int64_t state = token_state(p, w.item, w.kv_head, row);
 #pragma unroll
             for (int d = 0; d < Rows::ND; ++d)
-                *reinterpret_cast<f32x4*>(p.numerator + state * D + 16 * d + 4 * quad) = rows.o[r][d] * p.v_scale;
+                *reinterpret_cast<f32x4*>(p.numerator + state * D + rows.piece_dim(d, lane)) = rows.piece(r, d) * p.v_scale;
             if (quad == 0) *reinterpret_cast<float2*>(p.stats + state * 2) = make_float2(rows.m[r], sum);
         }
     }
@@ -720,7 +780,7 @@ __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const Token
         // Requests behind the end have no rows: they write zeros that nothing reads, and keep the counts the same.
         wait_for_loads<Load::NL>();  // all but V's
         const int later_ids = tile_pages<KT>(p, pages, t0 + 2 * step, lane);
-        rows.score(k_tile, s, lane);
+        rows.score(k_at, s, lane);
         wait_for_reads();
         k_load.request(p, next_ids, k_head, k_at, t0 + step, w.end, 0, lane);
         rows.weigh(s, t0, masked, invalid, p.scale_log2, lane);
@@ -730,7 +790,7 @@ __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const Token
                 bad |= holds_nonfinite<QT, KVF>(*reinterpret_cast<const u32x4*>(v_tile + i * 16));
             if (__any(bad)) break;
         }
-        rows.add(v_tile, s, lane);
+        rows.add(v_at, s, lane);
         wait_for_reads();
         v_load.request(p, next_ids, v_head, v_at, t0 + step, w.end, 0, lane);
         ids = next_ids;
@@ -748,10 +808,10 @@ __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const Token
     const int col = lane % 16, quad = lane / 16;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const float sum = sum_over_lane_groups(rows.l[r]);
+        const float sum = rows.sum(r);
 #pragma unroll
         for (int d = 0; d < Rows::ND; ++d)
-            *reinterpret_cast<f32x4*>(sums + (r * 16 + col) * Shape::SD + 16 * d + 4 * quad) = rows.o[r][d];
+            *reinterpret_cast<f32x4*>(sums + (r * 16 + col) * Shape::SD + rows.piece_dim(d, lane)) = rows.piece(r, d);
         if (quad == 0) states[wave][r * 16 + col] = make_float2(rows.m[r], sum);
     }
     __syncthreads();

@@ -126,10 +126,10 @@ PD_HD int64_t token_q_row(const TokenParams& p, int b, int kv_head, int token, i
 // permuted so that neither the reads of one chunk of many rows (K) nor those
 // of neighbouring rows that are transposed together (V: pairs of chunks of four rows;
 // FP8 as stored: one chunk of four rows and of those 16 behind) meet in a bank.
-// The permutation of a row is its own inverse.
+// The permutation of a row is its own inverse, and that of 32 rows on (but for FP8 as stored: of 16) is the same.
 template <int kRowBytes, bool kFp8>
 PD_HD int token_slot_chunk(int r, int c) {
-    if (kRowBytes == 64) return c ^ (((r >> 2) ^ (r >> 4)) & 3);                                        // FP8, D 64
+    if (kRowBytes == 64) return c ^ ((r >> 2) & 3) ^ ((r >> 4) & 1);                                     // FP8, D 64
     if (kRowBytes == 128 && kFp8) return c ^ ((((r >> 1) & 3) << 1) | (((r >> 3) ^ (r >> 4)) & 1));     // FP8, D 128
     if (kRowBytes == 128) return c ^ ((((r >> 1) & 3) << 1) | ((r >> 3) & 1));                          // 16-bit, D 64
     if (kRowBytes == 256) return c ^ (((r & 7) << 1) | ((r >> 3) & 1));                                 // 16-bit D 128, FP32 D 64
@@ -155,8 +155,11 @@ struct TokenPlan {
 
 constexpr int kStreamMaxRows = 32;     // rows that the stream kernel takes
 constexpr int kStreamWaves = 8;        // waves of its workgroups (FP32 rows are twice as long: 4)
-constexpr int kTokenMinSplit = 128;    // cache tokens per split, at least
+// Cache tokens per split, at least: FP32 products take sixteen times as long (33 tokens of 2 sequences of 1000: 13.2 us, with
+// splits of 128 14.4), others pay more for the merge (256 new tokens, BF16: 15.5 us, with splits of 64 16.4).
+constexpr int token_min_split(int q_bytes) { return q_bytes == 4 ? 64 : 128; }
 constexpr int kTokenGroupsPerCu = 2;   // workgroups per CU that splits of the tile kernel aim at
+constexpr int kTokenLongContext = 4096;
 
 // Items of splits of `span` tokens.
 inline int64_t token_items(int split, const int32_t* bounds, int batch, int64_t bound, int64_t span) {
@@ -173,9 +176,22 @@ inline int64_t token_workgroups(const TokenPlan& t, int kv_heads) {
     return static_cast<int64_t>((t.items + kXcds - 1) / kXcds * kXcds) * (kv_heads / t.head_waves) * t.row_tiles;
 }
 
+// Whether tiles of the tile kernel have 128 rows rather than 64: a tile of K and V in LDS then serves twice the rows, but there
+// are half the workgroups. So where those of 128 rows fill the device (with D 64, whose products wait less on LDS, twice over), or do
+// so in splits of 512 tokens of a context that is long next to the new tokens. Measured, 64 / 128 rows, 32 heads on 8: BF16,
+// D 128, 1536 tokens at 8192 257 / 214 us, 512 at 4096 60 / 54, 1024 at 16384 339 / 291; 768 at 4096 77 / 85, 1024
+// at 1024 24 / 29; D 64, 512 at 4096 40 / 37, and 28 heads on 4, 5 sequences of 301 34 / 45.
+inline bool wide_token_tiles(int q_bytes, int head_dim, int batch, int tokens, int64_t rows, int kv_heads, int64_t bound,
+                             int64_t compute_units) {
+    if (rows <= 64 || (q_bytes == 4 && head_dim == 128)) return false;  // (whose states of 128 rows the registers do not hold)
+    const int64_t tiles = batch * kv_heads * ((rows + 127) / 128);
+    if (head_dim == 128 ? tiles > compute_units : tiles >= kTokenGroupsPerCu * compute_units) return true;
+    return bound >= 8 * static_cast<int64_t>(tokens) && tiles * (bound / 512) >= kTokenGroupsPerCu * compute_units;
+}
+
 // The launch without splits, and the workgroups that splits aim at.
 inline TokenPlan plan_whole_tokens(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads,
-                                   int compute_units, int64_t& wanted) {
+                                   int64_t bound, int compute_units, int64_t& wanted) {
     TokenPlan t{};
     const int64_t rows = static_cast<int64_t>(tokens) * (query_heads / kv_heads);
     t.stream = rows <= kStreamMaxRows;
@@ -184,7 +200,7 @@ inline TokenPlan plan_whole_tokens(int q_bytes, int head_dim, int batch, int tok
         t.waves = q_bytes == 4 && head_dim == 128 ? kStreamWaves / 2 : kStreamWaves;
         t.head_waves = kv_heads % 2 == 0 ? 2 : 1;
     } else {
-        t.tile_rows = rows <= 64 || (q_bytes == 4 && head_dim == 128) ? 64 : 128;
+        t.tile_rows = wide_token_tiles(q_bytes, head_dim, batch, tokens, rows, kv_heads, bound, compute_units) ? 128 : 64;
         t.waves = 4;
         t.head_waves = 1;
     }
@@ -202,15 +218,17 @@ inline TokenPlan plan_whole_tokens(int q_bytes, int head_dim, int batch, int tok
 inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads, int64_t bound,
                              const int32_t* bounds, int64_t max_states, int compute_units) {
     int64_t wanted;
-    TokenPlan t = plan_whole_tokens(q_bytes, head_dim, batch, tokens, query_heads, kv_heads, compute_units, wanted);
+    TokenPlan t = plan_whole_tokens(q_bytes, head_dim, batch, tokens, query_heads, kv_heads, bound, compute_units, wanted);
     const int64_t each = t.workgroups / batch;  // workgroups of an item
     const int64_t states = static_cast<int64_t>(kv_heads) * t.row_tiles * t.tile_rows;  // and its states
     int64_t limit = lmin(wanted / each, max_states / states);  // items that fit the device at once
     if (t.stream && limit > kXcds) limit -= limit % kXcds;     // and each of its XCDs
-    if (t.workgroups >= compute_units || limit <= batch) return t;
+    // A workgroup per CU leaves CUs waiting, but the merge costs more than that unless the context is long (two halves, and whole: 96
+    // rows of 128 heads at 1500 27.3 / 25.2 us; 4096 rows of 8 at 16384 291 / 336).
+    if (t.workgroups > compute_units || (t.workgroups == compute_units && bound < kTokenLongContext) || limit <= batch) return t;
     const int split = batch <= kTokenListBatch ? kTokenList : kTokenGrid;
     // The shortest split with which the items fit; more tokens, fewer of them.
-    int64_t low = kTokenMinSplit / kTokenSplitUnit, high = (bound + kTokenSplitUnit - 1) / kTokenSplitUnit;
+    int64_t low = token_min_split(q_bytes) / kTokenSplitUnit, high = (bound + kTokenSplitUnit - 1) / kTokenSplitUnit;
     while (low < high) {
         const int64_t mid = (low + high) / 2;
         if (token_items(split, bounds, batch, bound, mid * kTokenSplitUnit) <= limit) high = mid;
@@ -229,11 +247,11 @@ inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, i
 inline int64_t most_token_states(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads, int64_t reach,
                                  int compute_units) {
     int64_t most = 0;
-    for (int n = 1; n <= tokens && reach > kTokenMinSplit; ++n) {
+    for (int n = 1; n <= tokens && reach > token_min_split(q_bytes); ++n) {
         int64_t wanted;
-        const TokenPlan t = plan_whole_tokens(q_bytes, head_dim, batch, n, query_heads, kv_heads, compute_units, wanted);
-        if (t.workgroups >= compute_units && !t.stream) break;  // and so for every larger n
-        const int64_t items = lmin(wanted / (t.workgroups / batch), batch * ((reach + kTokenMinSplit - 1) / kTokenMinSplit));
+        const TokenPlan t = plan_whole_tokens(q_bytes, head_dim, batch, n, query_heads, kv_heads, reach, compute_units, wanted);
+        if (t.workgroups > compute_units && !t.stream) break;  // and so for every larger n
+        const int64_t items = lmin(wanted / (t.workgroups / batch), batch * ((reach + token_min_split(q_bytes) - 1) / token_min_split(q_bytes)));
         if (items > batch) most = lmax(most, items * kv_heads * t.row_tiles * t.tile_rows);
     }
     return most;
