@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const Token
     TokenWork w;
     int last;
     if (!open_work<M>(p, at, w, last, lane)) {  // the same for all waves
-        if (p.split == kTokenWhole)
+        if (p.split == kTokenWhole && at.item < p.items)  // not the empty ones behind the last item, which have no rows
             for (int i = slice; i < M; i += slices) store_row_zeros<QT, D>(p, w, w.row0 + i, lane);
         return;
     }

@@ -280,3 +280,20 @@ def test_refusals():
         plan.run_tokens(q, k, v, out=torch.empty_like(q, dtype=torch.float32))
     with pytest.raises(ValueError):
         plan.run_tokens(q, k, v, out=q)
+
+
+@pytest.mark.parametrize("batch", [1, 3, 7])
+def test_short_calls_repeat_bit_for_bit(batch):
+    """Items are dealt to eight groups of workgroups; those without an item may not touch the last sequence's rows, whenever
+    they run."""
+    announce(f"repeated short calls of {batch} sequences")
+    layout = Layout(batch, 8, 4, 64, 16, 4 * batch)
+    table, q, k, v = problem(layout, torch.bfloat16, torch.bfloat16, 1, 4, seed=31)
+    lengths = np.full(batch, 64, dtype=np.int32)
+    plan = DecodePlan(layout, table, lengths, query_tokens=1)
+    first = plan.run_tokens(q, k, v)
+    check(layout, table, lengths, None, q, k, v, first, True)
+    outs = torch.full((4000, *q.shape), float("nan"), device="cuda", dtype=q.dtype)
+    for out in outs:
+        plan.run_tokens(q, k, v, out=out)
+    assert torch.equal(outs.view(torch.int16), first.view(torch.int16).expand(outs.shape))
