@@ -16,6 +16,20 @@ int launch_tokens_bf16_d128(const TokenParams&, const TokenPlan&, int kv_dtype, 
 // Splits of a sequence, on average, up to which a wave merges a row.
 constexpr int kMergeWaveSplits = 12;
 
+template <typename QT, int D>
+int merge_tokens(const TokenParams& p, hipStream_t stream) {
+    if (p.split != kTokenWhole) {
+        const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens * p.query_heads;
+        // Four waves for a row of many splits, where one would read them in turns.
+        if (p.items > kMergeWaveSplits * p.batch) {
+            hipLaunchKernelGGL((token_merge_kernel<QT, D, 4>), dim3(static_cast<uint32_t>(rows)), dim3(256), 0, stream, p);
+        } else {
+            hipLaunchKernelGGL((token_merge_kernel<QT, D, 1>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream, p);
+        }
+    }
+    return hipGetLastError() == hipSuccess ? PD_OK : PD_ERR_LAUNCH;
+}
+
 template <typename QT, int KVF, int D>
 int launch_tokens_format(const TokenParams& p, const TokenPlan& plan, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(token_workgroups(plan, p.kv_heads)));
@@ -30,18 +44,15 @@ int launch_tokens_format(const TokenParams& p, const TokenPlan& plan, hipStream_
     } else if (plan.tile_rows == 64) {
         hipLaunchKernelGGL((token_kernel<QT, KVF, D, 1, 4, KT>), grid, dim3(4 * kWave), 0, stream, p);
     } else if constexpr (!(sizeof(QT) == 4 && D == 128)) {
+        if constexpr (D == 128) {
+            if (plan.products_first) {
+                hipLaunchKernelGGL((token_kernel<QT, KVF, D, 2, 4, KT, true>), grid, dim3(4 * kWave), 0, stream, p);
+                return merge_tokens<QT, D>(p, stream);
+            }
+        }
         hipLaunchKernelGGL((token_kernel<QT, KVF, D, 2, 4, KT>), grid, dim3(4 * kWave), 0, stream, p);
     }
-    if (p.split != kTokenWhole) {
-        const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens * p.query_heads;
-        // Four waves for a row of many splits, where one would read them in turns.
-        if (p.items > kMergeWaveSplits * p.batch) {
-            hipLaunchKernelGGL((token_merge_kernel<QT, D, 4>), dim3(static_cast<uint32_t>(rows)), dim3(256), 0, stream, p);
-        } else {
-            hipLaunchKernelGGL((token_merge_kernel<QT, D, 1>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream, p);
-        }
-    }
-    return hipGetLastError() == hipSuccess ? PD_OK : PD_ERR_LAUNCH;
+    return merge_tokens<QT, D>(p, stream);
 }
 
 template <typename QT, int D>
