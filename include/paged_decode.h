@@ -434,6 +434,7 @@ int pd_append_rotated_advance(const pd_rotation* rotation, const pd_token_rows* 
  * rows over long contexts need to fill the device; with less than
  * pd_decode_tokens_workspace reports the call splits less and is slower. It
  * needs no initialisation; calls that overlap must not share one.
+ * hints: as in pd_decode_ex; PD_HINT_RAGGED_LENGTHS changes nothing here.
  * length_bounds: NULL, or a HOST array [batch] of upper bounds on the lengths,
  * read during the call, from which the split is chosen. Bounds below the
  * device lengths are still correct, only slower. No counterpart in the
@@ -442,7 +443,7 @@ int pd_append_rotated_advance(const pd_rotation* rotation, const pd_token_rows* 
 int pd_decode_tokens(const void* q, int q_dtype, const void* k, const void* v, int kv_dtype, float k_scale,
                      float v_scale, const int32_t* table, const int32_t* lengths, const int32_t* counts, void* out,
                      void* workspace, size_t workspace_bytes, int batch, int tokens, int query_heads, int kv_heads,
-                     int head_dim, int page_size, int table_width, int physical_pages, int causal,
+                     int head_dim, int page_size, int table_width, int physical_pages, int causal, int hints,
                      const int32_t* length_bounds, void* stream);
 
 /*

@@ -85,7 +85,7 @@ PROTOTYPES = {
     "pd_append_rotated": (_I, [_ROTATION, _ROWS, _ROWS, _ROWS, _I, _P, _P, _P, _P, _P, _P, _I, _F, _F] + [_I] * 8 + [_P]),
     "pd_append_rotated_advance": (_I, [_ROTATION, _ROWS, _ROWS, _ROWS, _I, _P, _P, _P, _P, _P, _P, _I, _F, _F] +
                                   [_I] * 9 + [_P]),
-    "pd_decode_tokens": (_I, [_P, _I, _P, _P, _I, _F, _F, _P, _P, _P, _P, _P, ctypes.c_size_t] + [_I] * 9 + [_P, _P]),
+    "pd_decode_tokens": (_I, [_P, _I, _P, _P, _I, _F, _F, _P, _P, _P, _P, _P, ctypes.c_size_t] + [_I] * 10 + [_P, _P]),
     "pd_decode_tokens_workspace": (ctypes.c_size_t, [_I] * 10),
     "pd_workspace_bytes": (ctypes.c_size_t, [_I] * 4),
     "pd_decode_launch_count": (_I, [_I] * 12 + [_P]),

@@ -221,14 +221,21 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const char* base, u
 // registers. In assembly since the compiler, where it knows of such a load, waits for it
 // before the next read of any LDS; here wait_for_loads and a barrier come
 // before the tile's first read. Nothing is returned in registers.
-template <int kOffset>
+// kOnce: past the caches, for what is read once.
+template <int kOffset, bool kOnce>
 __device__ __forceinline__ void load_to_lds(const char* base, uint32_t bytes, uint32_t to, uint32_t offset) {
     const uint64_t at = reinterpret_cast<uint64_t>(base);
     const u32x4 buffer = {static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32) & 0xFFFFu, bytes, 0x00027000u};
-    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
-                 :
-                 : "s"(to), "i"(kOffset), "v"(offset), "s"(buffer)
-                 : "memory", "scc");
+    if constexpr (kOnce)
+        asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen nt lds"
+                     :
+                     : "s"(to), "i"(kOffset), "v"(offset), "s"(buffer)
+                     : "memory", "scc");
+    else
+        asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
+                     :
+                     : "s"(to), "i"(kOffset), "v"(offset), "s"(buffer)
+                     : "memory", "scc");
 }
 
 // All loads of this wave but the last kNewer have arrived, those into LDS too.
@@ -257,7 +264,7 @@ __device__ __forceinline__ RowBlock row_block(const TokenParams& p, int page, in
 // A tile of KT cache tokens of K or V on its way into LDS, by WAVES waves. It
 // goes there directly, as stored, or (kWiden, FP8) through registers, where it is
 // widened when it lands.
-template <typename QT, int KVF, int D, int WAVES, int KT, bool kWiden>
+template <typename QT, int KVF, int D, int WAVES, int KT, bool kWiden, bool kOnce>
 struct TileLoad {
     static constexpr bool kFp8 = KVF != kTokenNative;
     static constexpr int SB = D * (kFp8 ? 1 : static_cast<int>(sizeof(QT)));            // bytes of a row in the cache
@@ -295,7 +302,7 @@ struct TileLoad {
         } else {
             // LDS slot `lane` of the request holds the chunk that token_chunk puts there.
             const uint32_t offset = r * p.kv_row_bytes + token_slot_chunk<RB, kFp8>(16 * block + r, lane % LPR) * 16;
-            load_to_lds<kPart * RPI * RB>(head + rows.offset, rows.bytes, to, offset);
+            load_to_lds<kPart * RPI * RB, kOnce>(head + rows.offset, rows.bytes, to, offset);
         }
     }
 
@@ -623,7 +630,7 @@ __device__ __forceinline__ bool open_work(const TokenParams& p, const TokenCoord
 template <typename QT, int KVF, int D, int R, int WAVES, int KT, bool kProductsFirst = false>
 __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenParams p) {
     using Rows = TokenRowsState<QT, kTokenNative, D, R>;
-    using Load = TileLoad<QT, KVF, D, WAVES, KT, KVF != kTokenNative>;
+    using Load = TileLoad<QT, KVF, D, WAVES, KT, KVF != kTokenNative, false>;
     constexpr int RB = Rows::RB;
     constexpr int M = WAVES * R * 16;
     constexpr int TILE = KT * RB;
@@ -729,7 +736,9 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
 // Few rows: every wave streams cache tokens of its own, tiles of 32 or 64 from
 // its part of LDS, for all R blocks of 16 rows, and the workgroup's waves of
 // one KV head combine at the end. The next K is requested once a tile is scored,
-// the next V once it is added, so that a wave always has loads in flight.
+// the next V once it is added, so that a wave always has loads in flight. kOnce:
+// no page is read by two sequences, and K and V stream past the caches (us with, without: FP16, 64 sequences
+// of 2048 87.7, 98.9, 32 of up to 4096 67.6, 76.5, 4 of 4096 22.8, 23.7; E4M3, 16 of up to 8192 46.4, 49.5; one of 8192 18.4, 17.8).
 template <typename QT, int KVF, int D, int R, int WAVES>
 struct StreamShape {
     static constexpr int SB = D * (KVF == kTokenNative ? static_cast<int>(sizeof(QT)) : 1);
@@ -740,12 +749,12 @@ struct StreamShape {
     static constexpr int REGION = 2 * TILE > STATE ? 2 * TILE : STATE;
 };
 
-template <typename QT, int KVF, int D, int R, int WAVES>
+template <typename QT, int KVF, int D, int R, int WAVES, bool kOnce>
 __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const TokenParams p) {
     using Rows = TokenRowsState<QT, KVF, D, R>;
     using Shape = StreamShape<QT, KVF, D, R, WAVES>;
     constexpr int KT = Shape::KT;
-    using Load = TileLoad<QT, KVF, D, 1, KT, false>;
+    using Load = TileLoad<QT, KVF, D, 1, KT, false, kOnce>;
     constexpr int M = R * 16;
     __shared__ __attribute__((aligned(1024))) char regions[WAVES * Shape::REGION];
     __shared__ float2 states[WAVES][M];

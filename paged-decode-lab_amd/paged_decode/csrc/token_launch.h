@@ -36,10 +36,13 @@ int launch_tokens_format(const TokenParams& p, const TokenPlan& plan, hipStream_
     constexpr int KT = sizeof(QT) == 4 ? 32 : 64;
     if (plan.stream) {
         constexpr int WAVES = sizeof(QT) == 4 && D == 128 ? kStreamWaves / 2 : kStreamWaves;
+        const dim3 threads(WAVES * kWave);
         if (plan.tile_rows == 16) {
-            hipLaunchKernelGGL((token_stream_kernel<QT, KVF, D, 1, WAVES>), grid, dim3(WAVES * kWave), 0, stream, p);
+            if (plan.once) hipLaunchKernelGGL((token_stream_kernel<QT, KVF, D, 1, WAVES, true>), grid, threads, 0, stream, p);
+            else hipLaunchKernelGGL((token_stream_kernel<QT, KVF, D, 1, WAVES, false>), grid, threads, 0, stream, p);
         } else {
-            hipLaunchKernelGGL((token_stream_kernel<QT, KVF, D, 2, WAVES>), grid, dim3(WAVES * kWave), 0, stream, p);
+            if (plan.once) hipLaunchKernelGGL((token_stream_kernel<QT, KVF, D, 2, WAVES, true>), grid, threads, 0, stream, p);
+            else hipLaunchKernelGGL((token_stream_kernel<QT, KVF, D, 2, WAVES, false>), grid, threads, 0, stream, p);
         }
     } else if (plan.tile_rows == 64) {
         hipLaunchKernelGGL((token_kernel<QT, KVF, D, 1, 4, KT>), grid, dim3(4 * kWave), 0, stream, p);

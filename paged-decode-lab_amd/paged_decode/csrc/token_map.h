@@ -152,6 +152,7 @@ struct TokenPlan {
     int tile_rows, row_tiles;
     int waves, head_waves;   // of a workgroup; stream kernel: KV heads among them
     bool products_first;     // tile kernel of 128 rows: see there
+    bool once;               // stream kernel: see there; the caller's to set
     int split, items, split_tokens;
     int64_t workgroups;  // with whole contexts
     int64_t states;      // 0 with whole contexts

@@ -57,7 +57,7 @@ size_t pd_decode_tokens_workspace(int q_dtype, int kv_dtype, int batch, int toke
 int pd_decode_tokens(const void* q, int q_dtype, const void* k, const void* v, int kv_dtype, float k_scale,
                      float v_scale, const int32_t* table, const int32_t* lengths, const int32_t* counts, void* out,
                      void* workspace, size_t workspace_bytes, int batch, int tokens, int query_heads, int kv_heads,
-                     int head_dim, int page_size, int table_width, int physical_pages, int causal,
+                     int head_dim, int page_size, int table_width, int physical_pages, int causal, int hints,
                      const int32_t* length_bounds, void* stream) {
     using namespace pd;
     if (!q || !k || !v || !table || !lengths || !out || (!workspace && workspace_bytes > 0)) return PD_ERR_NULL_POINTER;
@@ -65,6 +65,7 @@ int pd_decode_tokens(const void* q, int q_dtype, const void* k, const void* v, i
     if (!(k_scale > 0.0f && k_scale - k_scale == 0.0f && v_scale > 0.0f && v_scale - v_scale == 0.0f)) return PD_ERR_DTYPE;
     if (!token_shape(batch, tokens, query_heads, kv_heads, head_dim, page_size, table_width) || physical_pages < 1)
         return PD_ERR_SHAPE;
+    if ((hints & ~(PD_HINT_UNSHARED_PAGES | PD_HINT_RAGGED_LENGTHS)) != 0) return PD_ERR_HINT;
     if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(workspace)) return PD_ERR_SHAPE;
     // Rows of one (sequence, KV head) and bytes of a cache row are 32-bit numbers.
     const int64_t rows = static_cast<int64_t>(tokens) * (query_heads / kv_heads);
@@ -77,8 +78,9 @@ int pd_decode_tokens(const void* q, int q_dtype, const void* k, const void* v, i
         bound = std::min(std::max<int64_t>(bound, 1), reach);
     }
     const int64_t max_states = static_cast<int64_t>(workspace_bytes / state_bytes(head_dim));
-    const TokenPlan plan = plan_tokens(q_dtype == PD_DTYPE_F32 ? 4 : 2, head_dim, batch, tokens, query_heads, kv_heads, bound,
+    TokenPlan plan = plan_tokens(q_dtype == PD_DTYPE_F32 ? 4 : 2, head_dim, batch, tokens, query_heads, kv_heads, bound,
                                        length_bounds, max_states, device_cus());
+    plan.once = (hints & PD_HINT_UNSHARED_PAGES) != 0;
     if (token_workgroups(plan, kv_heads) > 0x7FFFFFFF || static_cast<int64_t>(batch) * tokens * query_heads > 0x7FFFFFFFLL * 4) return PD_ERR_SHAPE;
 
     TokenParams p{};

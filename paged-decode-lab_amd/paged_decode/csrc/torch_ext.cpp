@@ -613,7 +613,7 @@ OptTensor append_rotated(std::tuple<int64_t, int64_t, int64_t, int64_t, int64_t,
 torch::Tensor decode_tokens(std::tuple<int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> layout, torch::Tensor q,
                             torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lengths, OptTensor counts,
                             OptTensor given, torch::Tensor own, torch::Tensor workspace, bool causal, double k_scale,
-                            double v_scale, OptTensor length_bounds) {
+                            double v_scale, bool unshared_pages, OptTensor length_bounds) {
     const auto [batch, query_heads, kv_heads, dim, page_size, pages] = layout;
     PD_VALUE(q.dim() == 4 && q.size(0) == batch && q.size(1) >= 1 && q.size(1) <= own.size(1) && q.size(2) == query_heads && q.size(3) == dim,
              "input shape does not match plan");
@@ -649,7 +649,8 @@ torch::Tensor decode_tokens(std::tuple<int64_t, int64_t, int64_t, int64_t, int64
                                   lengths.data_ptr<int32_t>(), count, out.data_ptr(), bytes > 0 ? workspace.data_ptr() : nullptr,
                                   bytes, static_cast<int>(batch), static_cast<int>(q.size(1)), static_cast<int>(query_heads),
                                   static_cast<int>(kv_heads), static_cast<int>(dim), static_cast<int>(page_size),
-                                  static_cast<int>(table.size(1)), static_cast<int>(pages), causal, bounds, current_stream(q)));
+                                  static_cast<int>(table.size(1)), static_cast<int>(pages), causal,
+                                  unshared_pages ? PD_HINT_UNSHARED_PAGES : PD_HINT_NONE, bounds, current_stream(q)));
     return out;
 }
 

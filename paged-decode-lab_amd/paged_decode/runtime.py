@@ -311,7 +311,7 @@ class DecodePlan:
             raise ValueError("the plan reserves no query tokens: build it with query_tokens")
         return self._extension.decode_tokens(dimensions(self.layout), q, k, v, self._table, self._lengths, counts, out,
                                              self._token_out, self._token_workspace, causal, k_scale, v_scale,
-                                             self._length_bounds())
+                                             self._unshared_pages, self._length_bounds())
 
     def launches(self, q_dtype, kv_dtype=None):
         """Kernel launches ``run`` makes for q (and K/V) of these dtypes: 1 when the

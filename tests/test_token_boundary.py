@@ -86,7 +86,7 @@ def test_append_refuses_contexts_beyond_the_limit(most):
 
 def tokens_call(lib, **over):
     a = dict(q=FAKE, qt=cabi.PD_DTYPE_F16, k=FAKE, v=FAKE, kt=cabi.PD_DTYPE_F16, ks=1.0, vs=1.0, table=FAKE, lengths=FAKE, counts=None,
-             out=FAKE, ws=None, size=0, batch=2, tokens=3, hq=4, hkv=2, d=64, page=16, width=4, pages=8, causal=1)
+             out=FAKE, ws=None, size=0, batch=2, tokens=3, hq=4, hkv=2, d=64, page=16, width=4, pages=8, causal=1, hints=0)
     a.update(over)
     return lib.pd_decode_tokens(*a.values(), None, None)
 
@@ -99,6 +99,7 @@ def tokens_call(lib, **over):
     (dict(tokens=0), cabi.PD_ERR_SHAPE), (dict(tokens=65536), cabi.PD_ERR_SHAPE), (dict(hq=5), cabi.PD_ERR_SHAPE), (dict(hkv=0), cabi.PD_ERR_SHAPE),
     (dict(d=32), cabi.PD_ERR_SHAPE), (dict(page=64), cabi.PD_ERR_SHAPE), (dict(width=65537), cabi.PD_ERR_SHAPE), (dict(pages=0), cabi.PD_ERR_SHAPE),
     (dict(q=FAKE + 2), cabi.PD_ERR_SHAPE), (dict(tokens=65535, hq=65535, hkv=1), cabi.PD_ERR_SHAPE),
+    (dict(hints=4), cabi.PD_ERR_HINT),
 ])
 def test_token_attention_refusals(over, status):
     assert tokens_call(cabi.load(), **over) == status
