@@ -164,7 +164,11 @@ constexpr int kStreamWaves = 8;        // waves of its workgroups (FP32 rows are
 // splits of 128 14.4), others pay more for the merge (256 new tokens, BF16: 15.5 us, with splits of 64 16.4).
 constexpr int token_min_split(int q_bytes) { return q_bytes == 4 ? 64 : 128; }
 constexpr int kTokenGroupsPerCu = 2;   // workgroups per CU that splits of the tile kernel aim at
-constexpr int kTokenLongContext = 4096;
+// What splits cost, in cache tokens of a tile (of FP32 an eighth of as many): the merge's launch, and floats of states per token. Where
+// two workgroups share a CU a token counts one and a half. Splits by this rule, and against it (us, 32 heads on 8, FP16): 300 tokens on a
+// sequence of 600 whole 16.7, split 21.6; 256 on 256 8.8, 15.8; one on 200 9.0, 11.4; 16 x 2 on 600 split 16.8, whole 19.5; BF16, 512 on
+// 4096 53.4, 67.0; 1024 on 16384 260, 310. With D 64, 16 heads on 16, 8 x 96 on 1500 whole 25.0, split 27.3.
+constexpr int kTokenMergeCost = 280, kTokenStateCost = 128 * 120;
 
 // Items of splits of `span` tokens.
 inline int64_t token_items(int split, const int32_t* bounds, int batch, int64_t bound, int64_t span) {
@@ -229,9 +233,7 @@ inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, i
     const int64_t states = static_cast<int64_t>(kv_heads) * t.row_tiles * t.tile_rows;  // and its states
     int64_t limit = lmin(wanted / each, max_states / states);  // items that fit the device at once
     if (t.stream && limit > kXcds) limit -= limit % kXcds;     // and each of its XCDs
-    // A workgroup per CU leaves CUs waiting, but the merge costs more than that unless the context is long (two halves, and whole: 96
-    // rows of 128 heads at 1500 27.3 / 25.2 us; 4096 rows of 8 at 16384 291 / 336).
-    if (t.workgroups > compute_units || (t.workgroups == compute_units && bound < kTokenLongContext) || limit <= batch) return t;
+    if (t.workgroups > compute_units || limit <= batch) return t;
     const int split = batch <= kTokenListBatch ? kTokenList : kTokenGrid;
     // The shortest split with which the items fit; more tokens, fewer of them.
     int64_t low = token_min_split(q_bytes) / kTokenSplitUnit, high = (bound + kTokenSplitUnit - 1) / kTokenSplitUnit;
@@ -240,8 +242,19 @@ inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, i
         if (token_items(split, bounds, batch, bound, mid * kTokenSplitUnit) <= limit) high = mid;
         else low = mid + 1;
     }
-    const int64_t span = low * kTokenSplitUnit;
-    if (span >= bound) return t;
+    // That, or of longer ones the cheapest, or none.
+    int64_t best = bound, span = 0;
+    for (int64_t x = low * kTokenSplitUnit; x < bound; x *= 2) {
+        const int64_t items = token_items(split, bounds, batch, bound, x);
+        const bool shared = !t.stream && items * each > compute_units;  // CUs by two workgroups, each then slower
+        const int64_t fast = q_bytes == 4 ? 8 : 1;
+        const int64_t cost = (shared ? x * 3 / 2 : x) + (kTokenMergeCost + items * states * head_dim / kTokenStateCost) / fast;
+        if (cost < best) {
+            best = cost;
+            span = x;
+        }
+    }
+    if (span == 0) return t;
     t.split = split;
     t.split_tokens = static_cast<int>(span);
     t.items = static_cast<int>(token_items(split, bounds, batch, bound, span));
