@@ -278,23 +278,23 @@ struct TileLoad {
     static_assert(!kWiden || kFp8, "what is widened");
     u32x4 raw[kWiden ? NL : 1];
 
-    // ids: tile_pages of the tile; head: the cache from its KV head on; to: the tile's address in LDS.
-    __device__ __forceinline__ void request(const TokenParams& p, int ids, const char* head, uint32_t to, int t0, int end,
-                                            int wave, int lane) {
-        request_part(std::make_integer_sequence<int, NL>{}, p, ids, head, to + wave * (RPW * RB), t0, end, wave, lane);
+    // ids: the tile's page ids, from lane first_id on; head: the cache from its KV head on; to: the tile's address in LDS.
+    __device__ __forceinline__ void request(const TokenParams& p, int ids, int first_id, const char* head, uint32_t to, int t0,
+                                            int end, int wave, int lane) {
+        request_part(std::make_integer_sequence<int, NL>{}, p, ids, first_id, head, to + wave * (RPW * RB), t0, end, wave, lane);
     }
 
     template <int... kParts>
-    __device__ __forceinline__ void request_part(std::integer_sequence<int, kParts...>, const TokenParams& p, int ids,
+    __device__ __forceinline__ void request_part(std::integer_sequence<int, kParts...>, const TokenParams& p, int ids, int first_id,
                                                  const char* head, uint32_t to, int t0, int end, int wave, int lane) {
-        (request_one<kParts>(p, ids, head, to, t0, end, wave, lane), ...);
+        (request_one<kParts>(p, ids, first_id, head, to, t0, end, wave, lane), ...);
     }
 
     template <int kPart>
-    __device__ __forceinline__ void request_one(const TokenParams& p, int ids, const char* head, uint32_t to, int t0, int end,
-                                                int wave, int lane) {
+    __device__ __forceinline__ void request_one(const TokenParams& p, int ids, int first_id, const char* head, uint32_t to, int t0,
+                                                int end, int wave, int lane) {
         const int block = wave * RPW / 16 + kPart * RPI / 16;
-        const RowBlock rows = row_block(p, __builtin_amdgcn_readlane(ids, block), t0 + 16 * block, end);
+        const RowBlock rows = row_block(p, __builtin_amdgcn_readlane(ids, first_id + block), t0 + 16 * block, end);
         const int r = wave * RPW % 16 + kPart * RPI % 16 + lane / LPR;
         if constexpr (kWiden) {
             const uint32_t offset = r * p.kv_row_bytes + (lane % LPR) * 16;
@@ -368,6 +368,14 @@ struct TokenRowsState {
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[r][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
+    }
+
+    // q is in its registers: no later read of it waits, and with it for whatever has been requested since.
+    __device__ __forceinline__ void arrive() {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[r][s]));
     }
 
     // Where the lane reads in a tile at `tile` in LDS: bases that constants are added to from one block of tokens to the next.
@@ -656,8 +664,8 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
     int ids = tile_pages<KT>(p, pages, w.begin, lane);
     uint32_t invalid = invalid_blocks<KT>(p, ids, w.begin, w.end, lane);
     const uint32_t k_at = lds_address(k_tiles), v_at = lds_address(v_tiles);
-    k_load.request(p, ids, k_head, k_at, w.begin, w.end, wave, lane);
-    v_load.request(p, ids, v_head, v_at, w.begin, w.end, wave, lane);
+    k_load.request(p, ids, 0, k_head, k_at, w.begin, w.end, wave, lane);
+    v_load.request(p, ids, 0, v_head, v_at, w.begin, w.end, wave, lane);
     ids = tile_pages<KT>(p, pages, w.begin + KT, lane);
     Rows rows;
     rows.open(p, w, w.row0 + wave * R * 16, lane);
@@ -674,8 +682,8 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
         const uint32_t here = invalid;
         // Behind the end the request has no rows: it writes zeros that nothing reads.
         invalid = invalid_blocks<KT>(p, ids, t0 + KT, w.end, lane);
-        k_load.request(p, ids, k_head, k_at + (buffer ^ 1) * TILE, t0 + KT, w.end, wave, lane);
-        v_load.request(p, ids, v_head, v_at + (buffer ^ 1) * TILE, t0 + KT, w.end, wave, lane);
+        k_load.request(p, ids, 0, k_head, k_at + (buffer ^ 1) * TILE, t0 + KT, w.end, wave, lane);
+        v_load.request(p, ids, 0, v_head, v_at + (buffer ^ 1) * TILE, t0 + KT, w.end, wave, lane);
         ids = tile_pages<KT>(p, pages, t0 + 2 * KT, lane);
         if (t0 + KT > common) {  // uniform
             bool bad = false;
@@ -736,24 +744,48 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
 // Few rows: every wave streams cache tokens of its own, tiles of 32 or 64 from
 // its part of LDS, for all R blocks of 16 rows, and the workgroup's waves of
 // one KV head combine at the end. The next K is requested once a tile is scored,
-// the next V once it is added, so that a wave always has loads in flight. kOnce:
+// the next V once it is added, so that a wave always has loads in flight, and nothing else in the loop waits
+// for loads: q and the page ids of many tiles are there before (with an id load in each step, which drains the others: E4M3, 64 x 4
+// tokens of up to 4096 76.6 us, without 72.6; FP32, 8 x 2 at 2048 34.1, 31.6). kOnce:
 // no page is read by two sequences, and K and V stream past the caches (us with, without: FP16, 64 sequences
 // of 2048 87.7, 98.9, 32 of up to 4096 67.6, 76.5, 4 of 4096 22.8, 23.7; E4M3, 16 of up to 8192 46.4, 49.5; one of 8192 18.4, 17.8).
 template <typename QT, int KVF, int D, int R, int WAVES>
 struct StreamShape {
     static constexpr int SB = D * (KVF == kTokenNative ? static_cast<int>(sizeof(QT)) : 1);
-    static constexpr int KT = SB >= 256 ? 32 : 64;  // so that a wave's tile of K and V is 8 to 32 KB
+    // A wave's tile of K and V is 8 to 32 KB. Half the tile in rings of two is slower where it costs anything (E4M3, 16 x 8 tokens of up
+    // to 8192 47.3 us, with one of each 45.4; 64 x 4 of up to 4096 77.9, 72.6; BF16 the same): every tile has its scalar work.
+    static constexpr int KT = SB >= 256 ? 32 : 64;
     static constexpr int TILE = KT * SB;
     static constexpr int SD = D + 4;  // floats from one row's sums to the next: rows begin in other banks
     static constexpr int STATE = R * 16 * SD * 4;
     static constexpr int REGION = 2 * TILE > STATE ? 2 * TILE : STATE;
 };
 
+// Page ids of a wave's next tiles of NB blocks of 16 tokens, a block a lane: tiles of every `step`
+// tokens from t on. Here, and not where they are used, the wave waits for them, and with them for all that it requested.
+template <int NB>
+struct PageIds {
+    int ids;
+    uint64_t invalid;  // blocks on invalid pages
+
+    __device__ __forceinline__ void load(const TokenParams& p, const int32_t* pages, int t, int step, int end, int lane) {
+        const int token = t + lane / NB * step + 16 * (lane % NB);
+        ids = pages[imin(token >> p.page_shift, p.table_width - 1)];
+        asm volatile("" : "+v"(ids));
+        invalid = __ballot(static_cast<uint32_t>(ids) >= static_cast<uint32_t>(p.physical_pages) && token < end);
+    }
+
+    __device__ __forceinline__ uint32_t invalid_of(int tile) const {
+        return static_cast<uint32_t>(invalid >> (tile * NB)) & ((1u << NB) - 1);
+    }
+};
+
 template <typename QT, int KVF, int D, int R, int WAVES, bool kOnce>
 __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const TokenParams p) {
     using Rows = TokenRowsState<QT, KVF, D, R>;
     using Shape = StreamShape<QT, KVF, D, R, WAVES>;
-    constexpr int KT = Shape::KT;
+    constexpr int KT = Shape::KT, TILE = Shape::TILE;
+    constexpr int NB = KT / 16, TILES = kWave / NB;  // blocks of a tile; tiles whose page ids a wave holds
     using Load = TileLoad<QT, KVF, D, 1, KT, false, kOnce>;
     constexpr int M = R * 16;
     __shared__ __attribute__((aligned(1024))) char regions[WAVES * Shape::REGION];
@@ -775,42 +807,43 @@ __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const Token
     const char* k_head = static_cast<const char*>(p.k) + static_cast<size_t>(w.kv_head) * Load::SB;
     const char* v_head = static_cast<const char*>(p.v) + static_cast<size_t>(w.kv_head) * Load::SB;
     const int32_t* pages = p.table + static_cast<int64_t>(w.b) * p.table_width;
-    char* k_tile = regions + wave * Shape::REGION;
-    char* v_tile = k_tile + Shape::TILE;
-    const uint32_t k_at = lds_address(regions) + wave * Shape::REGION, v_at = k_at + Shape::TILE;
+    char* region = regions + wave * Shape::REGION;  // K's tile, and V's
+    const uint32_t k_at = lds_address(regions) + wave * Shape::REGION, v_at = k_at + TILE;
     const int step = slices * KT;
     const int first = w.begin + slice * KT;
 
-    Load k_load, v_load;
-    int ids = tile_pages<KT>(p, pages, first, lane);
-    int next_ids = tile_pages<KT>(p, pages, first + step, lane);
-    k_load.request(p, ids, k_head, k_at, first, w.end, 0, lane);
-    v_load.request(p, ids, v_head, v_at, first, w.end, 0, lane);
+    Load load;
     Rows rows;
     rows.open(p, w, w.row0, lane);
+    PageIds<NB> pages_of;
+    pages_of.load(p, pages, first, step, w.end, lane);
+    rows.arrive();
+    load.request(p, pages_of.ids, 0, k_head, k_at, first, w.end, 0, lane);
+    load.request(p, pages_of.ids, 0, v_head, v_at, first, w.end, 0, lane);
+    uint32_t invalid = pages_of.invalid_of(0);
+    int slot = 0;
     bool bad = false;
     for (int t0 = first; t0 < w.end; t0 += step) {
-        const uint32_t invalid = invalid_blocks<KT>(p, ids, t0, w.end, lane);
         const bool masked = t0 + KT > common || invalid != 0 || partial;
         f32x4 s[R][KT / 16];
         // Requests behind the end have no rows: they write zeros that nothing reads, and keep the counts the same.
         wait_for_loads<Load::NL>();  // all but V's
-        const int later_ids = tile_pages<KT>(p, pages, t0 + 2 * step, lane);
         rows.score(k_at, s, lane);
         wait_for_reads();
-        k_load.request(p, next_ids, k_head, k_at, t0 + step, w.end, 0, lane);
+        slot = (slot + 1) % TILES;
+        if (slot == 0) pages_of.load(p, pages, t0 + step, step, w.end, lane);
+        load.request(p, pages_of.ids, slot * NB, k_head, k_at, t0 + step, w.end, 0, lane);
         rows.weigh(s, t0, masked, invalid, p.scale_log2, lane);
         wait_for_loads<Load::NL>();  // all but the next K's
         if (t0 + KT > common) {
-            for (int i = lane; i < Shape::TILE / 16; i += kWave)
-                bad |= holds_nonfinite<QT, KVF>(*reinterpret_cast<const u32x4*>(v_tile + i * 16));
+            for (int i = lane; i < TILE / 16; i += kWave)
+                bad |= holds_nonfinite<QT, KVF>(*reinterpret_cast<const u32x4*>(region + TILE + i * 16));
             if (__any(bad)) break;
         }
         rows.add(v_at, s, lane);
         wait_for_reads();
-        v_load.request(p, next_ids, v_head, v_at, t0 + step, w.end, 0, lane);
-        ids = next_ids;
-        next_ids = later_ids;
+        load.request(p, pages_of.ids, slot * NB, v_head, v_at, t0 + step, w.end, 0, lane);
+        invalid = pages_of.invalid_of(slot);
     }
     wait_for_loads();
     const TokenParams late = reloaded_params();
@@ -820,7 +853,7 @@ __global__ void __launch_bounds__(kWave * WAVES) token_stream_kernel(const Token
     }
 
     // The waves' states, into their own parts of LDS.
-    float* sums = reinterpret_cast<float*>(k_tile);
+    float* sums = reinterpret_cast<float*>(region);
     const int col = lane % 16, quad = lane / 16;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
