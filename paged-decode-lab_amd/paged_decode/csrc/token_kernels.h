@@ -550,6 +550,30 @@ struct TokenRowsState {
         return kF32 ? i / 4 * 64 + lane / 16 * 16 + i % 4 * 4 : 16 * i + lane / 16 * 4;
     }
 
+    // The state in LDS, and the other group's of the same rows joined to this one's.
+    __device__ __forceinline__ void put(f32x4* to) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d) to[(r * (ND + 2) + d) * kWave] = o[r][d];
+            to[(r * (ND + 2) + ND) * kWave] = l[r];
+            to[(r * (ND + 2) + ND + 1) * kWave] = f32x4{m[r], most[r], 0.0f, 0.0f};
+        }
+    }
+    __device__ __forceinline__ void join(const f32x4* from) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const f32x4 head = from[(r * (ND + 2) + ND + 1) * kWave];
+            const bool here = most[r] > -INFINITY, there = head[1] > -INFINITY;  // whether they saw any token
+            const float top = fmaxf(here ? m[r] : kNoToken, there ? head[0] : kNoToken);
+            const float a = here ? fast_exp2(m[r] - top) : 0.0f, b = there ? fast_exp2(head[0] - top) : 0.0f;
+            m[r] = top;
+            l[r] = l[r] * a + from[(r * (ND + 2) + ND) * kWave] * b;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[r][d] = o[r][d] * a + from[(r * (ND + 2) + d) * kWave] * b;
+        }
+    }
+
     // A row's sum of weights, in all of its lanes.
     __device__ __forceinline__ float sum(int r) const {
         if constexpr (kF32) return sum_over_lane_groups((l[r][0] + l[r][1]) + (l[r][2] + l[r][3]));
@@ -631,27 +655,30 @@ __device__ __forceinline__ bool open_work(const TokenParams& p, const TokenCoord
 // ---------------------------------------------------------------------------
 // Many rows: a workgroup of WAVES waves, R blocks of 16 rows each, over tiles of
 // KT cache tokens that the waves share through LDS, two of them so that the
-// next is on its way while one is used. kProductsFirst: waves at their products
+// next is on its way while one is used. With two GROUPS of such waves each takes
+// every other tile into LDS of its own, and the states are joined at the end: where there is no more than one workgroup of 64 rows for a
+// CU, and not so few that splits fill the device (us with two, one: FP16, D 64, 8 x 96 on 1500 22.6, 25.6; D 128, 300 on 600
+// 14.9, 16.6; FP32, 2 x 200 on 1000 80, 87; but 64 on 300, in splits, 11.0, 10.3). kProductsFirst: waves at their products
 // come before those at their weights, so that the two waves of a SIMD fall out of step and one's products run beside the other's
 // weights. That takes many equal steps: BF16, D 128, 2048 tokens at 8192 227 us with it, 239 without, 1024 at 16384 260 and 288; but
 // whole prompts of 2048, where workgroups end at different times, 58.5 and 54.7.
-template <typename QT, int KVF, int D, int R, int WAVES, int KT, bool kProductsFirst = false>
-__global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenParams p) {
+template <typename QT, int KVF, int D, int R, int WAVES, int KT, int GROUPS, bool kProductsFirst>
+__global__ void __launch_bounds__(kWave * WAVES * GROUPS, 2) token_kernel(const TokenParams p) {
     using Rows = TokenRowsState<QT, kTokenNative, D, R>;
     using Load = TileLoad<QT, KVF, D, WAVES, KT, KVF != kTokenNative, false>;
     constexpr int RB = Rows::RB;
     constexpr int M = WAVES * R * 16;
     constexpr int TILE = KT * RB;
-    __shared__ __attribute__((aligned(1024))) char k_tiles[2 * TILE];
-    __shared__ __attribute__((aligned(1024))) char v_tiles[2 * TILE];
+    __shared__ __attribute__((aligned(1024))) char tiles[GROUPS * 4 * TILE];  // of each group two of K, two of V
 
     const int lane = threadIdx.x % kWave;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int group = any_wave / WAVES, wave = any_wave % WAVES;
     TokenWork w;
     int last;
     if (!open_work<M>(p, token_coords(p, blockIdx.x), w, last, lane)) {
         if (p.split == kTokenWhole)  // states of such splits are never read
-            for (int i = wave; i < M; i += WAVES) store_row_zeros<QT, D>(p, w, w.row0 + i, lane);
+            for (int i = any_wave; i < M; i += WAVES * GROUPS) store_row_zeros<QT, D>(p, w, w.row0 + i, lane);
         return;
     }
     // Cache tokens that every live row of the tile sees.
@@ -661,33 +688,37 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
     const char* v_head = static_cast<const char*>(p.v) + static_cast<size_t>(w.kv_head) * Load::SB;
     const int32_t* pages = p.table + static_cast<int64_t>(w.b) * p.table_width;
     Load k_load, v_load;
-    int ids = tile_pages<KT>(p, pages, w.begin, lane);
-    uint32_t invalid = invalid_blocks<KT>(p, ids, w.begin, w.end, lane);
-    const uint32_t k_at = lds_address(k_tiles), v_at = lds_address(v_tiles);
-    k_load.request(p, ids, 0, k_head, k_at, w.begin, w.end, wave, lane);
-    v_load.request(p, ids, 0, v_head, v_at, w.begin, w.end, wave, lane);
-    ids = tile_pages<KT>(p, pages, w.begin + KT, lane);
+    constexpr int STEP = GROUPS * KT;
+    const int first = w.begin + group * KT;
+    int ids = tile_pages<KT>(p, pages, first, lane);
+    uint32_t invalid = invalid_blocks<KT>(p, ids, first, w.end, lane);
+    char* own = tiles + group * 4 * TILE;
+    const uint32_t k_at = lds_address(tiles) + group * 4 * TILE, v_at = k_at + 2 * TILE;
+    k_load.request(p, ids, 0, k_head, k_at, first, w.end, wave, lane);
+    v_load.request(p, ids, 0, v_head, v_at, first, w.end, wave, lane);
+    ids = tile_pages<KT>(p, pages, first + STEP, lane);
     Rows rows;
     rows.open(p, w, w.row0 + wave * R * 16, lane);
 
     int buffer = 0;
     bool one_by_one = false;
-    for (int t0 = w.begin; t0 < w.end; t0 += KT, buffer ^= 1) {
-        char* k_tile = k_tiles + buffer * TILE;
-        char* v_tile = v_tiles + buffer * TILE;
+    for (int t = w.begin; t < w.end; t += STEP, buffer ^= 1) {
+        const int t0 = t + group * KT;
+        char* k_tile = own + buffer * TILE;
+        char* v_tile = own + (2 + buffer) * TILE;
         k_load.land(k_tile, wave, lane);
         v_load.land(v_tile, wave, lane);
         wait_for_loads();  // this wave's part of the tile is in LDS
         __syncthreads();   // everyone's part is, and the other tile is no longer read
         const uint32_t here = invalid;
         // Behind the end the request has no rows: it writes zeros that nothing reads.
-        invalid = invalid_blocks<KT>(p, ids, t0 + KT, w.end, lane);
-        k_load.request(p, ids, 0, k_head, k_at + (buffer ^ 1) * TILE, t0 + KT, w.end, wave, lane);
-        v_load.request(p, ids, 0, v_head, v_at + (buffer ^ 1) * TILE, t0 + KT, w.end, wave, lane);
-        ids = tile_pages<KT>(p, pages, t0 + 2 * KT, lane);
-        if (t0 + KT > common) {  // uniform
+        invalid = invalid_blocks<KT>(p, ids, t0 + STEP, w.end, lane);
+        k_load.request(p, ids, 0, k_head, k_at + (buffer ^ 1) * TILE, t0 + STEP, w.end, wave, lane);
+        v_load.request(p, ids, 0, v_head, v_at + (buffer ^ 1) * TILE, t0 + STEP, w.end, wave, lane);
+        ids = tile_pages<KT>(p, pages, t0 + 2 * STEP, lane);
+        if (t + STEP > common) {  // uniform
             bool bad = false;
-            for (int i = threadIdx.x; i < TILE / 16; i += WAVES * kWave)
+            for (int i = wave * kWave + lane; i < TILE / 16; i += WAVES * kWave)
                 bad |= holds_nonfinite<QT, kTokenNative>(*reinterpret_cast<const u32x4*>(v_tile + i * 16));
             bad = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad));  // known to be uniform: the loop's state stays in place
             if (bad) {
@@ -706,8 +737,17 @@ __global__ void __launch_bounds__(kWave * WAVES, 2) token_kernel(const TokenPara
     }
     wait_for_loads();  // the last request's: nothing may write LDS behind the workgroup's end
     if (one_by_one) {
-        token_rows_one_by_one<QT, KVF, D>(p, w, M, wave, WAVES, lane);
+        token_rows_one_by_one<QT, KVF, D>(p, w, M, any_wave, WAVES * GROUPS, lane);
         return;
+    }
+    if constexpr (GROUPS == 2) {
+        static_assert(WAVES * R * (Rows::ND + 2) * 1024 <= sizeof(tiles), "a group's state in place of the tiles");
+        __syncthreads();  // no tile is read any more
+        f32x4* state = reinterpret_cast<f32x4*>(tiles) + wave * R * (Rows::ND + 2) * kWave + lane;
+        if (group == 1) rows.put(state);
+        __syncthreads();
+        if (group == 1) return;
+        rows.join(state);
     }
 
     const int col = lane % 16, quad = lane / 16;

@@ -44,16 +44,18 @@ int launch_tokens_format(const TokenParams& p, const TokenPlan& plan, hipStream_
             if (plan.once) hipLaunchKernelGGL((token_stream_kernel<QT, KVF, D, 2, WAVES, true>), grid, threads, 0, stream, p);
             else hipLaunchKernelGGL((token_stream_kernel<QT, KVF, D, 2, WAVES, false>), grid, threads, 0, stream, p);
         }
-    } else if (plan.tile_rows == 64) {
-        hipLaunchKernelGGL((token_kernel<QT, KVF, D, 1, 4, KT>), grid, dim3(4 * kWave), 0, stream, p);
-    } else if constexpr (!(sizeof(QT) == 4 && D == 128)) {
-        if constexpr (D == 128) {
-            if (plan.products_first) {
-                hipLaunchKernelGGL((token_kernel<QT, KVF, D, 2, 4, KT, true>), grid, dim3(4 * kWave), 0, stream, p);
-                return merge_tokens<QT, D>(p, stream);
+    } else {
+        const dim3 threads(4 * kWave * plan.groups);
+        if (plan.tile_rows == 64) {
+            if (plan.groups == 2) hipLaunchKernelGGL((token_kernel<QT, KVF, D, 1, 4, KT, 2, false>), grid, threads, 0, stream, p);
+            else hipLaunchKernelGGL((token_kernel<QT, KVF, D, 1, 4, KT, 1, false>), grid, threads, 0, stream, p);
+        } else if constexpr (!(sizeof(QT) == 4 && D == 128)) {
+            if (D == 128 && plan.products_first) {
+                hipLaunchKernelGGL((token_kernel<QT, KVF, D, 2, 4, KT, 1, D == 128>), grid, threads, 0, stream, p);
+            } else {
+                hipLaunchKernelGGL((token_kernel<QT, KVF, D, 2, 4, KT, 1, false>), grid, threads, 0, stream, p);
             }
         }
-        hipLaunchKernelGGL((token_kernel<QT, KVF, D, 2, 4, KT>), grid, dim3(4 * kWave), 0, stream, p);
     }
     return merge_tokens<QT, D>(p, stream);
 }

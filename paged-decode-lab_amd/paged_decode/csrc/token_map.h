@@ -151,6 +151,7 @@ struct TokenPlan {
     bool stream;             // the kernel of few rows
     int tile_rows, row_tiles;
     int waves, head_waves;   // of a workgroup; stream kernel: KV heads among them
+    int groups;              // tile kernel: see there
     bool products_first;     // tile kernel of 128 rows: see there
     bool once;               // stream kernel: see there; the caller's to set
     int split, items, split_tokens;
@@ -167,7 +168,7 @@ constexpr int kTokenGroupsPerCu = 2;   // workgroups per CU that splits of the t
 // What splits cost, in cache tokens of a tile (of FP32 an eighth of as many): the merge's launch, and floats of states per token. Where
 // two workgroups share a CU a token counts one and a half. Splits by this rule, and against it (us, 32 heads on 8, FP16): 300 tokens on a
 // sequence of 600 whole 16.7, split 21.6; 256 on 256 8.8, 15.8; one on 200 9.0, 11.4; 16 x 2 on 600 split 16.8, whole 19.5; BF16, 512 on
-// 4096 53.4, 67.0; 1024 on 16384 260, 310. With D 64, 16 heads on 16, 8 x 96 on 1500 whole 25.0, split 27.3.
+// 4096 53.4, 67.0; 1024 on 16384 260, 310.
 constexpr int kTokenMergeCost = 280, kTokenStateCost = 128 * 120;
 
 // Items of splits of `span` tokens.
@@ -219,6 +220,7 @@ inline TokenPlan plan_whole_tokens(int q_bytes, int head_dim, int batch, int tok
     t.items = batch;
     t.split_tokens = 1 << 30;
     t.workgroups = static_cast<int64_t>(kv_heads / t.head_waves) * t.row_tiles * batch;
+    t.groups = !t.stream && t.tile_rows == 64 && t.workgroups <= compute_units && 2 * t.workgroups > compute_units ? 2 : 1;
     wanted = static_cast<int64_t>(compute_units) * (t.stream ? 1 : kTokenGroupsPerCu);
     return t;
 }
@@ -233,7 +235,7 @@ inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, i
     const int64_t states = static_cast<int64_t>(kv_heads) * t.row_tiles * t.tile_rows;  // and its states
     int64_t limit = lmin(wanted / each, max_states / states);  // items that fit the device at once
     if (t.stream && limit > kXcds) limit -= limit % kXcds;     // and each of its XCDs
-    if (t.workgroups > compute_units || limit <= batch) return t;
+    if (t.workgroups > compute_units || t.groups == 2 || limit <= batch) return t;
     const int split = batch <= kTokenListBatch ? kTokenList : kTokenGrid;
     // The shortest split with which the items fit; more tokens, fewer of them.
     int64_t low = token_min_split(q_bytes) / kTokenSplitUnit, high = (bound + kTokenSplitUnit - 1) / kTokenSplitUnit;
