@@ -1,4 +1,5 @@
 """Attention of several tokens per sequence on the GPU against 64-bit results (tests/rotary_oracle.py)."""
+import ctypes
 import math
 
 import numpy as np
@@ -11,6 +12,7 @@ require_gpu()
 import torch  # noqa: E402
 
 import rotary_oracle as oracle  # noqa: E402
+from paged_decode import cabi  # noqa: E402
 from paged_decode.layout import Layout  # noqa: E402
 from paged_decode.rotary import Rotary, append_rotated, rotate_heads  # noqa: E402
 from paged_decode.runtime import DecodePlan  # noqa: E402
@@ -297,3 +299,129 @@ def test_short_calls_repeat_bit_for_bit(batch):
     for out in outs:
         plan.run_tokens(q, k, v, out=out)
     assert torch.equal(outs.view(torch.int16), first.view(torch.int16).expand(outs.shape))
+
+
+# Which kernel a shape takes on 256 CUs: tiles of 64 rows by two groups of waves (129 to 256 of them), by one in splits, of 128 rows
+# (more than 256 of them, or long contexts) with short and with long contexts, in splits, and the grid of splits of more than 64
+# sequences by either kernel.
+SHAPES = [(5, 8, 8, 64, 300, 420), (5, 8, 8, 128, 290, 500), (3, 4, 1, 64, 40, 1900), (17, 8, 8, 128, 160, 200), (17, 8, 8, 128, 160, 420),
+          (17, 16, 16, 64, 150, 330), (2, 8, 8, 128, 160, 8200), (66, 2, 1, 128, 3, 1700), (70, 1, 1, 64, 40, 900)]
+
+
+@pytest.mark.parametrize("q_type,kv_type", [FORMATS[0], FORMATS[2], FORMATS[3]], ids=str)
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,tokens,context", SHAPES)
+def test_launches_of_every_kind(q_type, kv_type, batch, heads, kv_heads, dim, tokens, context):
+    announce(f"launch of {batch} x {tokens} on {context}, {heads}/{kv_heads} heads of {dim}, {q_type}/{kv_type}")
+    width = -(-context // 16)
+    layout = Layout(batch, heads, kv_heads, dim, 16, batch * width)
+    table, q, k, v = problem(layout, q_type, kv_type, tokens, width, seed=batch + dim)
+    rng = np.random.default_rng(context)
+    lengths = rng.integers(1, context + 1, size=batch).astype(np.int32)
+    lengths[0], lengths[-1] = context, 0
+    counts = rng.integers(0, tokens + 1, size=batch).astype(np.int32)
+    counts[0] = tokens
+    run(layout, table, lengths, q, k, v, counts=counts, causal=context % 200 != 0)
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,tokens,context", [SHAPES[0], SHAPES[1], SHAPES[4], SHAPES[6]])
+def test_hidden_nan_in_tiles_of_every_kind(batch, heads, kv_heads, dim, tokens, context):
+    """The last token's V is NaN: rows that do not see it are those of the clean cache, bit for bit or to rounding."""
+    announce(f"hidden NaN, {batch} x {tokens} on {context}")
+    width = -(-context // 16)
+    layout = Layout(batch, heads, kv_heads, dim, 16, batch * width)
+    table, q, k, v = problem(layout, torch.bfloat16, torch.bfloat16, tokens, width, seed=5)
+    lengths = np.full(batch, context, dtype=np.int32)
+    plan = DecodePlan(layout, table, lengths, query_tokens=tokens)
+    clean = plan.run_tokens(q, k, v).clone()
+    check(layout, table, lengths, None, q, k, v, clean, True)
+    at = (context - 1) // 16
+    for b in range(batch):
+        v[int(table[b, at]), (context - 1) % 16] = math.nan
+    out = plan.run_tokens(q, k, v)
+    assert not torch.isfinite(out[:, -1]).any()
+    v.nan_to_num_(0.0)
+    for b in (0, batch - 1):
+        keys, values = (gathered(x, table[b], context, 16) for x in (k, v))
+        sees = torch.arange(tokens, device="cuda") + context - tokens + 1
+        expected, bound = oracle.attention(q[b], keys, values, sees)
+        oracle.assert_within(out[b, :-1], expected[:-1], bound[:-1], q.dtype, f"sequence {b}")
+
+
+def test_two_graphs_of_one_plan_and_shared_pages():
+    """Graphs that share the plan's workspace, replayed in turn with eager calls between them; sequences that share their pages."""
+    announce("two graphs of a plan")
+    layout = Layout(3, 8, 2, 128, 16, 260)
+    table, _, k, v = problem(layout, torch.float16, torch.float16, 4, 80, seed=3)
+    table[1, :60] = table[0, :60]
+    lengths = np.array([1280, 1100, 961], dtype=np.int32)
+    plan = DecodePlan(layout, table, lengths, query_tokens=40)
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    q = [torch.randn((3, n, 8, 128), device="cuda", generator=gen).half() for n in (4, 40)]
+    outs = [torch.empty_like(x) for x in q]
+    graphs = []
+    for x, out in zip(q, outs):
+        plan.run_tokens(x, k, v, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan.run_tokens(x, k, v, out=out)
+        graphs.append(graph)
+    for step in range(6):
+        for x in q:
+            x.copy_(torch.randn(x.shape, device="cuda", generator=gen))
+        for graph in graphs if step % 2 else graphs[::-1]:
+            graph.replay()
+        eager = [plan.run_tokens(x, k, v, out=torch.empty_like(x)) for x in q]
+        torch.cuda.synchronize()
+        for x, out, own in zip(q, outs, eager):
+            assert torch.equal(out, own)
+            check(layout, table, lengths, None, x, k, v, out, True)
+
+
+def test_caches_past_32_bits():
+    """Pages that begin more than 2^32 bytes into a cache: written with rotation, and read by either kernel."""
+    announce("caches past 32 bits")
+    pages = (1 << 32) // (16 * 8 * 128 * 2) + 200
+    layout = Layout(1, 8, 8, 128, 16, pages)
+    table = (pages - 1 - np.arange(100, dtype=np.int32))[None].copy()
+    table[0, 1::2] = np.arange(50)
+    k, v = (torch.zeros((pages, 16, 8, 128), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    f = torch.pow(torch.tensor(10000.0, dtype=torch.float64), -torch.arange(64, dtype=torch.float64) / 64)
+    rotary = Rotary(f)
+    plan = DecodePlan(layout, table, np.zeros(1, dtype=np.int32), max_context=1600, query_tokens=1500)
+    q, k_new, v_new = (torch.randn((1, 1500, 8, 128), device="cuda", generator=gen).bfloat16() for _ in range(3))
+    rotated = plan.append_rotated(k, v, k_new, v_new, rotary, q=q)
+    lengths = np.array([1500], dtype=np.int32)
+    q_exact, k_exact = rotate_heads(q, k_new, torch.zeros(1, dtype=torch.int32, device="cuda"), rotary)
+    assert torch.equal(rotated, q_exact)
+    assert torch.equal(gathered(k, table[0, :94], 1500, 16), k_exact[0].float())
+    assert torch.equal(gathered(v, table[0, :94], 1500, 16), v_new[0].float())
+    check(layout, table, lengths, None, rotated, k, v, plan.run_tokens(rotated, k, v), True)
+    last = rotated[:, -3:].contiguous()
+    check(layout, table, lengths, None, last, k, v, plan.run_tokens(last, k, v), True)
+
+
+@pytest.mark.parametrize("tokens", [2, 40])
+@pytest.mark.parametrize("part", [0.0, 0.3, 1.0, 3.0])
+def test_c_entry_with_less_and_more_workspace(tokens, part):
+    announce(f"C entry, {tokens} tokens, {part} of the workspace")
+    layout = Layout(2, 4, 2, 64, 16, 300)
+    table, q, k, v = problem(layout, torch.float16, torch.float16, tokens, 150, seed=6)
+    lengths = np.array([2400, 1999], dtype=np.int32)
+    lib = cabi.load()
+    size = lib.pd_decode_tokens_workspace(cabi.PD_DTYPE_F16, cabi.PD_DTYPE_F16, 2, tokens, 4, 2, 64, 16, 150, 0)
+    assert size > 0
+    size = int(size * part) // 16 * 16
+    room = torch.full((size + 64,), 0xA5, dtype=torch.uint8, device="cuda")
+    ids, lens = torch.from_numpy(table).cuda(), torch.from_numpy(lengths).cuda()
+    for hints in (0, cabi.PD_HINT_UNSHARED_PAGES, cabi.PD_HINT_RAGGED_LENGTHS):
+        out = torch.full_like(q, float("nan"))
+        status = lib.pd_decode_tokens(q.data_ptr(), cabi.PD_DTYPE_F16, k.data_ptr(), v.data_ptr(), cabi.PD_DTYPE_F16, 1.0, 1.0,
+                                      ids.data_ptr(), lens.data_ptr(), None, out.data_ptr(), room.data_ptr() if size else None, size,
+                                      2, tokens, 4, 2, 64, 16, 150, 300, 1, hints, None,
+                                      ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert status == cabi.PD_OK
+        check(layout, table, lengths, None, q, k, v, out, True)
+    assert bool((room[size:] == 0xA5).all())
+
