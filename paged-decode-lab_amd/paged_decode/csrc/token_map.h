@@ -11,6 +11,8 @@
 
 #include <stddef.h>
 
+#include <initializer_list>
+
 #include "partition_map.h"
 
 namespace pd {
@@ -159,7 +161,12 @@ struct TokenPlan {
     int64_t states;      // 0 with whole contexts
 };
 
-constexpr int kStreamMaxRows = 32;     // rows that the stream kernel takes
+// Rows that the stream kernel takes: up to 16, and up to 32 where the tokens of all sequences and KV heads come to kStreamLoad per CU or
+// q is FP32. Below, the tile kernel's splits have fewer states to merge (us of FP16, 32 heads on 8, stream / tile: 8 x 8
+// tokens of 4096 37 / 34, 16 x 8 of 1024 27.8 / 25.0, 2 x 5 of 1000 15.4 / 10.8; 16 x 8 of 4096 55.8 / 57.7, 40 x 8 of 1500 48.8 /
+// 55.9; BF16, 12 x 8 of 8192 74.7 / 81.4; FP32, 16 x 5 of 2000 58 / 84).
+constexpr int kStreamMaxRows = 32;
+constexpr int kStreamLoad = 1600;
 constexpr int kStreamWaves = 8;        // waves of its workgroups (FP32 rows are twice as long: 4)
 // Cache tokens per split, at least: FP32 products take sixteen times as long (33 tokens of 2 sequences of 1000: 13.2 us, with
 // splits of 128 14.4), others pay more for the merge (256 new tokens, BF16: 15.5 us, with splits of 64 16.4).
@@ -204,7 +211,7 @@ inline TokenPlan plan_whole_tokens(int q_bytes, int head_dim, int batch, int tok
                                    int64_t bound, int compute_units, int64_t& wanted) {
     TokenPlan t{};
     const int64_t rows = static_cast<int64_t>(tokens) * (query_heads / kv_heads);
-    t.stream = rows <= kStreamMaxRows;
+    t.stream = rows <= 16 || (rows <= kStreamMaxRows && (q_bytes == 4 || batch * kv_heads * bound >= kStreamLoad * static_cast<int64_t>(compute_units)));
     if (t.stream) {
         t.tile_rows = rows <= 16 ? 16 : 32;
         t.waves = q_bytes == 4 && head_dim == 128 ? kStreamWaves / 2 : kStreamWaves;
@@ -264,16 +271,23 @@ inline TokenPlan plan_tokens(int q_bytes, int head_dim, int batch, int tokens, i
     return t;
 }
 
-// States with which no call of up to `tokens` tokens splits less than it would with more.
+// States with which no call of up to `tokens` tokens splits less than it would with more, whatever its lengths: with
+// the kernels of short and of long contexts.
 inline int64_t most_token_states(int q_bytes, int head_dim, int batch, int tokens, int query_heads, int kv_heads, int64_t reach,
                                  int compute_units) {
+    const int64_t splits = (reach + token_min_split(q_bytes) - 1) / token_min_split(q_bytes);
     int64_t most = 0;
-    for (int n = 1; n <= tokens && reach > token_min_split(q_bytes); ++n) {
-        int64_t wanted;
-        const TokenPlan t = plan_whole_tokens(q_bytes, head_dim, batch, n, query_heads, kv_heads, reach, compute_units, wanted);
-        if (t.workgroups > compute_units && !t.stream) break;  // and so for every larger n
-        const int64_t items = lmin(wanted / (t.workgroups / batch), batch * ((reach + token_min_split(q_bytes) - 1) / token_min_split(q_bytes)));
-        if (items > batch) most = lmax(most, items * kv_heads * t.row_tiles * t.tile_rows);
+    bool more = splits > 1;
+    for (int n = 1; n <= tokens && more; ++n) {
+        more = false;
+        for (const int64_t bound : {int64_t{1}, reach}) {
+            int64_t wanted;
+            const TokenPlan t = plan_whole_tokens(q_bytes, head_dim, batch, n, query_heads, kv_heads, bound, compute_units, wanted);
+            if (t.workgroups > compute_units && !t.stream) continue;  // and so for every larger n
+            more = true;
+            const int64_t items = lmin(wanted / (t.workgroups / batch), batch * splits);
+            if (items > batch) most = lmax(most, items * kv_heads * t.row_tiles * t.tile_rows);
+        }
     }
     return most;
 }

@@ -61,7 +61,7 @@ int main() {
         const TokenPlan t = plan_tokens(q_bytes, dim, batch, tokens, query, kv, bound, known ? bounds.data() : nullptr, states, cus);
         const int64_t rows = int64_t(tokens) * (query / kv);
         check(int64_t(t.row_tiles) * t.tile_rows >= rows && int64_t(t.row_tiles - 1) * t.tile_rows < rows);
-        check(t.stream == (rows <= kStreamMaxRows) && kv % t.head_waves == 0 && t.waves % t.head_waves == 0);
+        check((t.stream || rows > 16) && (!t.stream || rows <= kStreamMaxRows) && kv % t.head_waves == 0 && t.waves % t.head_waves == 0);
         check(q_bytes == 2 || dim == 64 || t.stream || t.tile_rows == 64);
         ++kinds[t.split], wide += t.tile_rows == 128, groups += t.groups == 2, streams += t.stream;
         TokenParams p{};
