@@ -346,8 +346,8 @@ int pd_table_from_csr(const int32_t* indptr, const int32_t* indices, int64_t ind
  * Weights are [head_dim], or [heads, head_dim] with *_weight_per_head; NULL: no
  * norm. weight_dtype is the tokens' dtype or PD_DTYPE_F32. frequencies and the
  * weights are device memory, weights aligned to 16 bytes; the struct itself is
- * read during the call. No counterpart in the reference, whose q and cache
- * rows arrive rotated (docs/DESIGN.md:10-13).
+ * read during the call. No counterpart in the reference, which
+ * leaves what is written to the cache to its caller (docs/DESIGN.md:11-13).
  */
 enum pd_rotate_style { PD_ROTATE_HALF = 0, PD_ROTATE_INTERLEAVED = 1 };
 

@@ -3,8 +3,8 @@
 ``rotate_heads`` norms and rotates new queries and keys; ``append_rotated``
 does so while it writes the keys, and the values beside them, into the cache
 (``DecodePlan.append_rotated`` at the plan's own lengths). The reference has
-neither: its q and cache rows arrive as attention reads them
-(docs/DESIGN.md:10-13).
+neither: it leaves what is written to the cache to its caller
+(docs/DESIGN.md:11-13).
 """
 import math
 
