@@ -378,7 +378,8 @@ typedef struct pd_token_rows {
  * q_out and k_out (F32, F16 or BF16, one dtype throughout; an output may be its
  * own contiguous input). positions is [batch] (token j of sequence b at
  * positions[b] + j), or [batch, tokens] if positions_per_token is not 0.
- * batch, tokens, heads <= 65535; head_dim 64 or 128.
+ * batch, tokens, heads <= 65535; head_dim 64 or 128; a call holds fewer than
+ * 2^26 groups of 512 dims of a token (more: PD_ERR_SHAPE).
  */
 int pd_rotate_heads(const pd_rotation* rotation, const pd_token_rows* q, const pd_token_rows* k, int dtype,
                     const int32_t* positions, int positions_per_token, void* q_out, void* k_out, int batch, int tokens,
@@ -426,7 +427,8 @@ int pd_append_rotated_advance(const pd_rotation* rotation, const pd_token_rows* 
  *   out[b, j, h] = softmax(k_scale K q / sqrt(head_dim)) (v_scale V)
  * over the tokens it sees, through KV head h / (query_heads / kv_heads). Rows
  * j >= c_b and rows that see no token are zeros. Formats, page ids and limits
- * as in pd_decode_ex; tokens <= 65535. Scores, softmax statistics and sums are
+ * as in pd_decode_ex; tokens <= 65535, and a launch of 2^32 threads at most
+ * (more: PD_ERR_SHAPE). Scores, softmax statistics and sums are
  * FP32; the weights enter the second product in q's type.
  *
  * workspace: NULL, or device memory of workspace_bytes (aligned to 16 bytes)

@@ -298,7 +298,7 @@ size_t type_size(int dtype) { return dtype == PD_DTYPE_F32 ? 4 : 2; }
 bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
 
 // 0 if the rows can be read 16 bytes at a time.
-int check_rows(const pd_token_rows* r, int dtype, int batch, int tokens, int heads, int head_dim) {
+int check_rows(const pd_token_rows* r, int dtype, int heads) {
     if (!r->data) return PD_ERR_NULL_POINTER;
     const int64_t unit = 16 / static_cast<int64_t>(type_size(dtype));
     if (misaligned(r->data) || r->batch_stride % unit != 0 || r->token_stride % unit != 0) return PD_ERR_SHAPE;
@@ -306,7 +306,6 @@ int check_rows(const pd_token_rows* r, int dtype, int batch, int tokens, int hea
     // Strides may be 0 (one row for several tokens), never negative; offsets stay far inside 63 bits.
     const int64_t limit = int64_t{1} << 40;
     if (r->batch_stride < 0 || r->token_stride < 0 || r->batch_stride > limit || r->token_stride > limit) return PD_ERR_SHAPE;
-    (void)batch, (void)tokens, (void)head_dim;
     return PD_OK;
 }
 
@@ -324,7 +323,7 @@ int check_rotation(const pd_rotation* r, int dtype, int head_dim) {
     return PD_OK;
 }
 
-RotateParams rotate_params(const pd_rotation* r, int dtype, int batch, int tokens, int head_dim) {
+RotateParams rotate_params(const pd_rotation* r, int batch, int tokens, int head_dim) {
     RotateParams p{};
     p.frequencies = r->frequencies;
     p.q_weight = r->q_weight;
@@ -340,7 +339,6 @@ RotateParams rotate_params(const pd_rotation* r, int dtype, int batch, int token
     p.weight_f32 = r->weight_dtype == PD_DTYPE_F32;
     p.q_weight_stride = r->q_weight_per_head ? head_dim : 0;
     p.k_weight_stride = r->k_weight_per_head ? head_dim : 0;
-    (void)dtype;
     return p;
 }
 
@@ -355,7 +353,8 @@ TokenRows token_rows(const pd_token_rows* r) {
 int plan_rotate(RotateParams& p, int head_dim) {
     const int hpw = rotate_heads_per_wave(head_dim);
     p.head_groups = (p.heads + hpw - 1) / hpw;
-    return static_cast<int64_t>(p.batch) * p.tokens * p.head_groups <= 0x7FFFFFFF ? PD_OK : PD_ERR_SHAPE;
+    // A launch holds 2^32 threads.
+    return static_cast<int64_t>(p.batch) * p.tokens * p.head_groups <= (int64_t{1} << 26) - kRotateWaves ? PD_OK : PD_ERR_SHAPE;
 }
 
 uint32_t rotate_blocks(const RotateParams& p) {
@@ -419,11 +418,11 @@ int append_rotated(const pd_rotation* rotation, const pd_token_rows* q, const pd
     if (advance && (max_context < 0 || max_context > (1 << 20))) return PD_ERR_SHAPE;
     if (misaligned(k_cache) || misaligned(v_cache) || misaligned(q_out)) return PD_ERR_SHAPE;
     int status = check_rotation(rotation, dtype, head_dim);
-    if (status == PD_OK && q) status = check_rows(q, dtype, batch, tokens, query_heads, head_dim);
-    if (status == PD_OK) status = check_rows(k, dtype, batch, tokens, kv_heads, head_dim);
-    if (status == PD_OK) status = check_rows(v, dtype, batch, tokens, kv_heads, head_dim);
+    if (status == PD_OK && q) status = check_rows(q, dtype, query_heads);
+    if (status == PD_OK) status = check_rows(k, dtype, kv_heads);
+    if (status == PD_OK) status = check_rows(v, dtype, kv_heads);
     if (status != PD_OK) return status;
-    RotateParams p = rotate_params(rotation, dtype, batch, tokens, head_dim);
+    RotateParams p = rotate_params(rotation, batch, tokens, head_dim);
     p.q = token_rows(q);
     p.k = token_rows(k);
     p.v = token_rows(v);
@@ -469,10 +468,10 @@ int pd_rotate_heads(const pd_rotation* rotation, const pd_token_rows* q, const p
     if (head_dim != 64 && head_dim != 128) return PD_ERR_SHAPE;
     if (misaligned(q_out) || misaligned(k_out)) return PD_ERR_SHAPE;
     int status = check_rotation(rotation, dtype, head_dim);
-    if (status == PD_OK) status = check_rows(q, dtype, batch, tokens, query_heads, head_dim);
-    if (status == PD_OK && k) status = check_rows(k, dtype, batch, tokens, kv_heads, head_dim);
+    if (status == PD_OK) status = check_rows(q, dtype, query_heads);
+    if (status == PD_OK && k) status = check_rows(k, dtype, kv_heads);
     if (status != PD_OK) return status;
-    RotateParams p = rotate_params(rotation, dtype, batch, tokens, head_dim);
+    RotateParams p = rotate_params(rotation, batch, tokens, head_dim);
     p.q = token_rows(q);
     p.k = token_rows(k);
     p.q_out = static_cast<char*>(q_out);

@@ -201,7 +201,7 @@ inline int64_t token_workgroups(const TokenPlan& t, int kv_heads) {
 inline bool wide_token_tiles(int q_bytes, int head_dim, int batch, int tokens, int64_t rows, int kv_heads, int64_t bound,
                              int64_t compute_units) {
     if (rows <= 64 || (q_bytes == 4 && head_dim == 128)) return false;  // (whose states of 128 rows the registers do not hold)
-    const int64_t tiles = batch * kv_heads * ((rows + 127) / 128);
+    const int64_t tiles = static_cast<int64_t>(batch) * kv_heads * ((rows + 127) / 128);
     if (head_dim == 128 ? tiles > compute_units : tiles >= kTokenGroupsPerCu * compute_units) return true;
     return bound >= 8 * static_cast<int64_t>(tokens) && tiles * (bound / 512) >= kTokenGroupsPerCu * compute_units;
 }
@@ -211,7 +211,7 @@ inline TokenPlan plan_whole_tokens(int q_bytes, int head_dim, int batch, int tok
                                    int64_t bound, int compute_units, int64_t& wanted) {
     TokenPlan t{};
     const int64_t rows = static_cast<int64_t>(tokens) * (query_heads / kv_heads);
-    t.stream = rows <= 16 || (rows <= kStreamMaxRows && (q_bytes == 4 || batch * kv_heads * bound >= kStreamLoad * static_cast<int64_t>(compute_units)));
+    t.stream = rows <= 16 || (rows <= kStreamMaxRows && (q_bytes == 4 || static_cast<int64_t>(batch) * kv_heads * bound >= kStreamLoad * static_cast<int64_t>(compute_units)));
     if (t.stream) {
         t.tile_rows = rows <= 16 ? 16 : 32;
         t.waves = q_bytes == 4 && head_dim == 128 ? kStreamWaves / 2 : kStreamWaves;

@@ -80,7 +80,7 @@ int pd_decode_tokens(const void* q, int q_dtype, const void* k, const void* v, i
     const int64_t max_states = static_cast<int64_t>(workspace_bytes / state_bytes(head_dim));
     TokenPlan plan = plan_tokens(q_dtype == PD_DTYPE_F32 ? 4 : 2, head_dim, batch, tokens, query_heads, kv_heads, bound,
                                        length_bounds, max_states, device_cus());
-    if (token_workgroups(plan, kv_heads) > 0x7FFFFFFF || static_cast<int64_t>(batch) * tokens * query_heads > 0x7FFFFFFFLL * 4) return PD_ERR_SHAPE;
+    if (token_workgroups(plan, kv_heads) * plan.waves * plan.groups * kWave > 0xFFFFFFFFLL) return PD_ERR_SHAPE;  // a launch's threads
 
     TokenParams p{};
     p.q = q;

@@ -45,6 +45,7 @@ def rotate(lib, rot=None, q=None, k=None, **over):
     (dict(rot=rotation(weight_dtype=cabi.PD_DTYPE_BF16)), cabi.PD_ERR_DTYPE),
     (dict(rot=rotation(eps=-1.0)), cabi.PD_ERR_SHAPE), (dict(rot=rotation(q_weight=FAKE + 2)), cabi.PD_ERR_SHAPE),
     (dict(q=cabi.TokenRows(None, 768, 256)), cabi.PD_ERR_NULL_POINTER), (dict(q=cabi.TokenRows(FAKE, 768, 260)), cabi.PD_ERR_SHAPE),
+    (dict(batch=65535, tokens=2048), cabi.PD_ERR_SHAPE),  # more threads than a launch holds
     (dict(q=cabi.TokenRows(FAKE + 4, 768, 256)), cabi.PD_ERR_SHAPE), (dict(k=cabi.TokenRows(FAKE, -384, 128)), cabi.PD_ERR_SHAPE),
 ])
 def test_rotation_refusals(over, status):
@@ -100,6 +101,7 @@ def tokens_call(lib, **over):
     (dict(d=32), cabi.PD_ERR_SHAPE), (dict(page=64), cabi.PD_ERR_SHAPE), (dict(width=65537), cabi.PD_ERR_SHAPE), (dict(pages=0), cabi.PD_ERR_SHAPE),
     (dict(q=FAKE + 2), cabi.PD_ERR_SHAPE), (dict(tokens=65535, hq=65535, hkv=1), cabi.PD_ERR_SHAPE),
     (dict(hints=4), cabi.PD_ERR_HINT),
+    (dict(batch=65535, tokens=1, hq=2048, hkv=2048), cabi.PD_ERR_SHAPE), (dict(batch=65535, tokens=65535, hq=64, hkv=64), cabi.PD_ERR_SHAPE),
 ])
 def test_token_attention_refusals(over, status):
     assert tokens_call(cabi.load(), **over) == status
