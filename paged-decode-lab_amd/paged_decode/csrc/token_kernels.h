@@ -655,13 +655,19 @@ __device__ __forceinline__ bool open_work(const TokenParams& p, const TokenCoord
 // ---------------------------------------------------------------------------
 // Many rows: a workgroup of WAVES waves, R blocks of 16 rows each, over tiles of
 // KT cache tokens that the waves share through LDS, two of them so that the
-// next is on its way while one is used. With two GROUPS of such waves each takes
-// every other tile into LDS of its own, and the states are joined at the end: where there is no more than one workgroup of 64 rows for a
-// CU, and not so few that splits fill the device (us with two, one: FP16, D 64, 8 x 96 on 1500 22.6, 25.6; D 128, 300 on 600
-// 14.9, 16.6; FP32, 2 x 200 on 1000 80, 87; but 64 on 300, in splits, 11.0, 10.3). kProductsFirst: waves at their products
-// come before those at their weights, so that the two waves of a SIMD fall out of step and one's products run beside the other's
-// weights. That takes many equal steps: BF16, D 128, 2048 tokens at 8192 227 us with it, 239 without, 1024 at 16384 260 and 288; but
-// whole prompts of 2048, where workgroups end at different times, 58.5 and 54.7.
+// next is on its way while one is used.
+// Two GROUPS of such waves take every other tile each, into LDS of their own, and
+// join their states at the end. That serves where there is no more than one workgroup of 64
+// rows per CU, but too many for splits (us with two groups, with one: FP16, D 64, 8 x
+// 96 tokens on 1500 22.6, 25.6; D 128, 300 on 600 14.9, 16.6; FP32, 2 x 200 on 1000
+// 80, 87; but 64 on 300, which splits serve, 11.0, 10.3).
+// kProductsFirst: waves at their products come before those at their weights, so that
+// the two waves of a SIMD fall out of step and one's products run beside the other's
+// weights. That takes many equal steps (us with it, without: BF16, D 128, 2048 tokens
+// on 8192 227, 239; 1024 on 16384 260, 288; but whole prompts of 2048, whose
+// workgroups end at different times, 58.5, 54.7).
+// What bounds it: at D 128 the matrix cores (54% busy on 2048 tokens at 8192, 92% of
+// a large product's rate in all) and the vector units that they share the SIMDs with.
 template <typename QT, int KVF, int D, int R, int WAVES, int KT, int GROUPS, bool kProductsFirst>
 __global__ void __launch_bounds__(kWave * WAVES * GROUPS, 2) token_kernel(const TokenParams p) {
     using Rows = TokenRowsState<QT, kTokenNative, D, R>;
@@ -784,16 +790,20 @@ __global__ void __launch_bounds__(kWave * WAVES * GROUPS, 2) token_kernel(const 
 // Few rows: every wave streams cache tokens of its own, tiles of 32 or 64 from
 // its part of LDS, for all R blocks of 16 rows, and the workgroup's waves of
 // one KV head combine at the end. The next K is requested once a tile is scored,
-// the next V once it is added, so that a wave always has loads in flight, and nothing else in the loop waits
-// for loads: q and the page ids of many tiles are there before (with an id load in each step, which drains the others: E4M3, 64 x 4
-// tokens of up to 4096 76.6 us, without 72.6; FP32, 8 x 2 at 2048 34.1, 31.6). kOnce:
-// no page is read by two sequences, and K and V stream past the caches (us with, without: FP16, 64 sequences
-// of 2048 87.7, 98.9, 32 of up to 4096 67.6, 76.5, 4 of 4096 22.8, 23.7; E4M3, 16 of up to 8192 46.4, 49.5; one of 8192 18.4, 17.8).
+// the next V once it is added, so that a wave always has loads in flight, and nothing
+// else in the loop waits for loads: q and the page ids of many tiles are there before
+// (us with ids loaded in each step, and so: E4M3, 64 x 4 tokens of up to 4096 76.6, 72.6;
+// FP32, 8 x 2 at 2048 34.1, 31.6).
+// kOnce: no page is read by two sequences, and K and V stream past the caches (us with,
+// without: FP16, 64 sequences of 2048 87.7, 98.9, 32 of up to 4096 67.6, 76.5, 4 of 4096
+// 22.8, 23.7; E4M3, 16 of up to 8192 46.4, 49.5).
+// What bounds it: memory where a wave has many steps (64 sequences of 2048: 6.4 TB/s);
+// with a few, the chain of lengths, page ids and first tiles, and the merge.
 template <typename QT, int KVF, int D, int R, int WAVES>
 struct StreamShape {
     static constexpr int SB = D * (KVF == kTokenNative ? static_cast<int>(sizeof(QT)) : 1);
-    // A wave's tile of K and V is 8 to 32 KB. Half the tile in rings of two is slower where it costs anything (E4M3, 16 x 8 tokens of up
-    // to 8192 47.3 us, with one of each 45.4; 64 x 4 of up to 4096 77.9, 72.6; BF16 the same): every tile has its scalar work.
+    // A wave's tile of K and V is 8 to 32 KB. Rings of two tiles half as long were slower (E4M3, 16 x 8 tokens of up
+    // to 8192 47.3 us, so 45.4; 64 x 4 of up to 4096 77.9, 72.6; BF16 the same): every tile has its scalar work.
     static constexpr int KT = SB >= 256 ? 32 : 64;
     static constexpr int TILE = KT * SB;
     static constexpr int SD = D + 4;  // floats from one row's sums to the next: rows begin in other banks

@@ -161,21 +161,25 @@ struct TokenPlan {
     int64_t states;      // 0 with whole contexts
 };
 
-// Rows that the stream kernel takes: up to 16, and up to 32 where the tokens of all sequences and KV heads come to kStreamLoad per CU or
-// q is FP32. Below, the tile kernel's splits have fewer states to merge (us of FP16, 32 heads on 8, stream / tile: 8 x 8
-// tokens of 4096 37 / 34, 16 x 8 of 1024 27.8 / 25.0, 2 x 5 of 1000 15.4 / 10.8; 16 x 8 of 4096 55.8 / 57.7, 40 x 8 of 1500 48.8 /
-// 55.9; BF16, 12 x 8 of 8192 74.7 / 81.4; FP32, 16 x 5 of 2000 58 / 84).
+// Rows that the stream kernel takes: up to 16, and up to 32 where the tokens of all sequences and KV heads come to
+// kStreamLoad per CU or q is FP32. Below, the tile kernel's splits have fewer states to merge (us, 32 heads on 8,
+// stream / tile: FP16, 8 x 8 tokens on 4096 37 / 34, 16 x 8 on 1024 27.8 / 25.0, 2 x 5 on 1000 15.4 / 10.8; 16 x 8 on
+// 4096 55.8 / 57.7, 40 x 8 on 1500 48.8 / 55.9; BF16, 12 x 8 on 8192 74.7 / 81.4; FP32, 16 x 5 on 2000 58 / 84).
 constexpr int kStreamMaxRows = 32;
 constexpr int kStreamLoad = 1600;
-constexpr int kStreamWaves = 8;        // waves of its workgroups (FP32 rows are twice as long: 4)
-// Cache tokens per split, at least: FP32 products take sixteen times as long (33 tokens of 2 sequences of 1000: 13.2 us, with
-// splits of 128 14.4), others pay more for the merge (256 new tokens, BF16: 15.5 us, with splits of 64 16.4).
+// Waves of its workgroups (FP32 rows of D 128 are twice as long: 4). With 4: FP32, 8 x 2 on 2048 34.6 us, with 8 31.5;
+// E4M3, 16 x 8 on up to 8192 44.4, 45.5; others the same.
+constexpr int kStreamWaves = 8;
+// Cache tokens per split, at least: FP32 products take sixteen times as long (2 x 33 tokens on 1000: 13.2 us, with
+// splits of 128 14.4), others pay more for the merge (BF16, 256 tokens on 256: 15.5 us, with splits of 64 16.4).
 constexpr int token_min_split(int q_bytes) { return q_bytes == 4 ? 64 : 128; }
-constexpr int kTokenGroupsPerCu = 2;   // workgroups per CU that splits of the tile kernel aim at
-// What splits cost, in cache tokens of a tile (of FP32 an eighth of as many): the merge's launch, and floats of states per token. Where
-// two workgroups share a CU a token counts one and a half. Splits by this rule, and against it (us, 32 heads on 8, FP16): 300 tokens on a
-// sequence of 600 whole 16.7, split 21.6; 256 on 256 8.8, 15.8; one on 200 9.0, 11.4; 16 x 2 on 600 split 16.8, whole 19.5; BF16, 512 on
-// 4096 53.4, 67.0; 1024 on 16384 260, 310.
+// Workgroups per CU that splits of the tile kernel aim at (FP16, 128 tokens on 16384: 65 us, with three 78).
+constexpr int kTokenGroupsPerCu = 2;
+// What splits cost, in cache tokens of a tile (of FP32 an eighth of as many): the merge's launch, and floats of states
+// per token. Where two workgroups share a CU a token counts one and a half. By this rule, and against it (us, 32 heads
+// on 8; FP16, 300 tokens on 600 whole 16.7, split 21.6; 256 on 256 whole 8.8, split 15.8; one on 200 whole 9.0, split
+// 11.4; 16 x 2 on 600 split 16.8, whole 19.5; BF16, 512 on 4096 in four splits 53.4, in two 67.0; 1024 on 16384 split
+// 291, whole 336).
 constexpr int kTokenMergeCost = 280, kTokenStateCost = 128 * 120;
 
 // Items of splits of `span` tokens.
@@ -193,11 +197,11 @@ inline int64_t token_workgroups(const TokenPlan& t, int kv_heads) {
     return static_cast<int64_t>((t.items + kXcds - 1) / kXcds * kXcds) * (kv_heads / t.head_waves) * t.row_tiles;
 }
 
-// Whether tiles of the tile kernel have 128 rows rather than 64: a tile of K and V in LDS then serves twice the rows, but there
-// are half the workgroups. So where those of 128 rows fill the device (with D 64, whose products wait less on LDS, twice over), or do
-// so in splits of 512 tokens of a context that is long next to the new tokens. Measured, 64 / 128 rows, 32 heads on 8: BF16,
-// D 128, 1536 tokens at 8192 257 / 214 us, 512 at 4096 60 / 54, 1024 at 16384 339 / 291; 768 at 4096 77 / 85, 1024
-// at 1024 24 / 29; D 64, 512 at 4096 40 / 37, and 28 heads on 4, 5 sequences of 301 34 / 45.
+// Whether tiles of the tile kernel have 128 rows rather than 64: a tile of K and V in LDS then serves twice the rows, but
+// there are half the workgroups. So where those of 128 rows fill the device (with D 64, whose products wait less on LDS,
+// twice over), or do so in splits of 512 tokens of a context that is long next to the new tokens. Measured, 64 / 128 rows,
+// 32 heads on 8: BF16, D 128, 1536 tokens on 8192 257 / 214 us, 512 on 4096 60 / 54, 1024 on 16384 339 / 291; 768 on 4096
+// 77 / 85, 1024 on 1024 24 / 29; D 64, 512 on 4096 40 / 37, and 28 heads on 4, 5 sequences of 301 34 / 45.
 inline bool wide_token_tiles(int q_bytes, int head_dim, int batch, int tokens, int64_t rows, int kv_heads, int64_t bound,
                              int64_t compute_units) {
     if (rows <= 64 || (q_bytes == 4 && head_dim == 128)) return false;  // (whose states of 128 rows the registers do not hold)
@@ -211,10 +215,13 @@ inline TokenPlan plan_whole_tokens(int q_bytes, int head_dim, int batch, int tok
                                    int64_t bound, int compute_units, int64_t& wanted) {
     TokenPlan t{};
     const int64_t rows = static_cast<int64_t>(tokens) * (query_heads / kv_heads);
-    t.stream = rows <= 16 || (rows <= kStreamMaxRows && (q_bytes == 4 || static_cast<int64_t>(batch) * kv_heads * bound >= kStreamLoad * static_cast<int64_t>(compute_units)));
+    const int64_t load = static_cast<int64_t>(batch) * kv_heads * bound / compute_units;  // cache tokens per CU
+    t.stream = rows <= 16 || (rows <= kStreamMaxRows && (q_bytes == 4 || load >= kStreamLoad));
     if (t.stream) {
         t.tile_rows = rows <= 16 ? 16 : 32;
         t.waves = q_bytes == 4 && head_dim == 128 ? kStreamWaves / 2 : kStreamWaves;
+        // Two KV heads' rows lie side by side (us with two, one: 64 sequences of 2048 83, 91; E4M3, 16 x 8 on up to 8192 45.5, 49.4;
+        // 4 x 4 on 4096 22.6, 21.0, one of 16384 19.5, 20.3).
         t.head_waves = kv_heads % 2 == 0 ? 2 : 1;
     } else {
         t.tile_rows = wide_token_tiles(q_bytes, head_dim, batch, tokens, rows, kv_heads, bound, compute_units) ? 128 : 64;
